@@ -657,6 +657,127 @@ int ob200_search_debug_record(ob200_search* s, const float** policy_out, const f
 int ob200_search_debug_phases(ob200_search* s, int32_t enable, double* phase_ms_out);
 int ob200_copy_to_host(void* dst_host, const void* src_device, int64_t bytes);
 
+/* ------------------------------------------------------------------------- *
+ *  Training operators: what a learner runs between the search's visit counts
+ *  and the next weights of a network.  The reference's learner
+ *  (alphazero_train.py, python/alphazero/alphazero_trainer.py) builds its loss
+ *  and its optimiser step from PyTorch's elementary operations; these are the
+ *  same kind of step as single launches over caller-owned DEVICE memory of the
+ *  current device, asynchronous on `stream`, capturable, without allocation.
+ *  Sums, softmax statistics and norms are held in 32 bits or more; results do
+ *  not depend on the order in which CTAs run.
+ * ------------------------------------------------------------------------- */
+#define OB200_DTYPE_F32 2       /* policy rows, gradients and weights only       */
+
+/* Rows of policy logits, one per position, with what every policy loss writes.
+ * An action counts as legal when its bit is set (legal_bits NULL: all are) and
+ * its logit is not -inf; the policy is the softmax over the legal actions, and
+ * what stands at other places (infinities and NaN included) is not looked at.
+ * A row is left out - loss, statistics and gradient are 0 - when its weight is 0
+ * (it is then not read), when it has no legal action, or for the reason its
+ * loss names.  A NaN or +inf logit of a legal action makes its row's results
+ * NaN.  Columns from n_actions to the pitch are neither read nor written. */
+typedef struct ob200_policy_rows {
+    const void* logits;         /* [n][logits_pitch] of dtype                     */
+    const uint32_t* legal_bits; /* [n][mask_words] as ob200_tree_view, or NULL    */
+    const float* row_weight;    /* [n] factor of each row's loss; NULL = all 1    */
+    void* grad;                 /* [n][grad_pitch] of dtype: d loss / d logits, 0 at
+                                   actions that are not legal.  May be `logits`
+                                   itself (same pitch)                            */
+    float* loss;                /* [n], or NULL                                   */
+    float* stats;               /* [n][4], 16-byte aligned, or NULL               */
+    int64_t logits_pitch;       /* elements between rows, >= n_actions            */
+    int64_t grad_pitch;
+    int32_t n;                  /* rows; 0 is a call without work                 */
+    int32_t n_actions;
+    int32_t mask_words;         /* >= ceil(n_actions / 32)                        */
+    int32_t dtype;              /* OB200_DTYPE_*                                  */
+} ob200_policy_rows;
+
+#define OB200_TARGET_VISITS 0   /* int32 visit counts                             */
+#define OB200_TARGET_PROBS 1    /* fp32, any positive scale                       */
+
+/* Cross entropy with the search's visit distribution:
+ *   pi = target / sum of target over the legal actions,  p = the policy,
+ *   loss = w * (- sum pi log p - entropy_coef * H(p)),  H(p) = - sum p log p
+ *   grad = w * (p - pi + entropy_coef * p * (log p + H))
+ *   stats = (cross entropy, H, sum of the target, log of the sum of exp(logit)).
+ * Targets are not negative.  A row whose target sums to 0 (no simulation reached
+ * a legal action) is left out. */
+int ob200_launch_policy_loss_search(const ob200_policy_rows* rows, const void* target, int64_t target_pitch,
+                                    int32_t target_kind, float entropy_coef, ob200_stream stream);
+
+/* Clipped-ratio policy loss with a KL term against a reference policy q (the
+ * softmax of ref_logits over the same legal actions):
+ *   r = exp(log p[action] - old_logp),  c = min(max(r, 1 - clip_low), 1 + clip_high)
+ *   loss = w * (- min(r * advantage, c * advantage) + kl_coef * KL - entropy_coef * H)
+ *   KL = sum p (log p - log q)
+ *   stats = (log p[action], r, KL, H).
+ * The gradient of the first term is that of r * advantage where it is not the
+ * larger one, 0 elsewhere; an advantage of 0 contributes 0 whatever r is.
+ * ref_logits may be NULL (KL = 0; kl_coef must then be 0).  A row whose action is
+ * outside [0, n_actions) or not legal is left out.  KL is not finite where q gives
+ * no probability to an action that p gives some. */
+int ob200_launch_policy_loss_clipped(const ob200_policy_rows* rows, const int32_t* action, const float* old_logp,
+                                     const float* advantage, const void* ref_logits, int64_t ref_pitch,
+                                     float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                                     ob200_stream stream);
+
+/* One trained tensor.  `tensors` arguments below are HOST arrays, read before the
+ * call returns; the memory they name belongs to the device.  Pointers need the
+ * alignment of their elements only (16-byte aligned tensors are faster). */
+typedef struct ob200_train_tensor {
+    void* param;                /* [numel] of param_dtype                         */
+    const void* grad;           /* [numel] of grad_dtype                          */
+    void* exp_avg;              /* [numel] first moment: fp32, or e4m3            */
+    void* exp_avg_sq;           /* [numel] second moment: fp32, or its root in e4m3 */
+    float* exp_avg_scale;       /* [ceil(numel / 256)], states in 8 bits only     */
+    float* exp_avg_sq_scale;
+    int64_t numel;              /* 0 is allowed                                   */
+    float weight_decay;
+} ob200_train_tensor;
+
+/* out[0] = 2-norm over the `grad` of all tensors (their other fields are not
+ * used), out[1] = the factor that clips it: max_norm / out[0] where out[0] >
+ * max_norm, else 1.  Squares are fp32: a gradient beyond 1.8e19 makes the norm
+ * infinite.  Where out[0] is not finite out[1] is NaN, which ob200_launch_adamw
+ * takes as "leave this step out".  `workspace`: DEVICE,
+ * ob200_grad_norm_workspace_bytes() bytes, 8-byte aligned, contents arbitrary;
+ * calls that may overlap need one each. */
+int64_t ob200_grad_norm_workspace_bytes(void);
+int ob200_launch_grad_norm(const ob200_train_tensor* tensors, int32_t n_tensors, int32_t grad_dtype, float max_norm,
+                           void* workspace, float* out, ob200_stream stream);
+
+typedef struct ob200_adamw_config {
+    double lr, beta1, beta2, eps;
+    int32_t step;               /* 1 for the first step                           */
+    int32_t param_dtype;        /* OB200_DTYPE_*                                  */
+    int32_t grad_dtype;
+    int32_t state_bits;         /* 32 or 8                                        */
+    const float* grad_scale;    /* DEVICE, or NULL: factor of every gradient.  When it
+                                   is not finite the call changes nothing         */
+    const float* lr_device;     /* DEVICE, or NULL: used in place of lr           */
+    const int32_t* step_device; /* DEVICE, or NULL: used in place of step (for
+                                   captured graphs)                               */
+} ob200_adamw_config;
+
+/* One AdamW step over all tensors, for each element, in fp32:
+ *   g = grad * grad_scale
+ *   m = beta1 * m + (1 - beta1) * g,   v = beta2 * v + (1 - beta2) * g^2
+ *   param = param * (1 - lr * weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+ * param is rounded once to its type; updates smaller than half a step of a
+ * 16-bit type are lost, so keep fp32 weights where that matters.
+ * state_bits 8: each run of 256 elements of a tensor shares an fp32 scale,
+ * max / 448 (maxima below 2^-110 count as 2^-110): the first moment is held as
+ * e4m3 times its scale, the second as the square of (e4m3 times its scale), a
+ * value above 0 never becoming 0.  The step itself uses m and v before they are
+ * rounded.  Zeroed codes and scales are the state before the first step.
+ * A moment that is not finite makes the states of its 256 elements NaN.
+ * No two tensors of a call may share memory (OB200_ERR_INVALID where params or
+ * states of one kind do). */
+int ob200_launch_adamw(const ob200_train_tensor* tensors, int32_t n_tensors, const ob200_adamw_config* cfg,
+                       ob200_stream stream);
+
 /* Per-device counters for the end-of-run reduction (the only cross-GPU step;
  * it replaces the MCTSStats fields total_evaluations / total_batches_processed,
  * include/mcts/mcts_engine.h:154-197). */

@@ -16,6 +16,9 @@ OUT_PROBS, OUT_LOGITS = 0, 1
 GUARD = 32
 RULES_FREESTYLE, RULES_OMOK, RULES_RENJU = 0, 1, 2
 DTYPE_BF16, DTYPE_F16 = 0, 1     # storage type of board tensors and packed tower weights
+DTYPE_F32 = 2                    # policy rows, gradients and weights of the training operators
+TARGET_VISITS, TARGET_PROBS = 0, 1
+ERR_INVALID = 1
 
 
 class Error(RuntimeError):
@@ -61,6 +64,23 @@ class SearchConfig(C.Structure):
 class SearchStats(C.Structure):
     _fields_ = [("simulations", C.c_int64), ("evaluations", C.c_int64), ("nodes", C.c_int64),
                 ("terminal_leaves", C.c_int64), ("device_ms", C.c_double), ("wall_ms", C.c_double)]
+
+
+class PolicyRows(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("legal_bits", C.c_void_p), ("row_weight", C.c_void_p), ("grad", C.c_void_p),
+                ("loss", C.c_void_p), ("stats", C.c_void_p), ("logits_pitch", C.c_int64), ("grad_pitch", C.c_int64),
+                ("n", C.c_int32), ("n_actions", C.c_int32), ("mask_words", C.c_int32), ("dtype", C.c_int32)]
+
+
+class TrainTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p), ("numel", C.c_int64), ("weight_decay", C.c_float)]
+
+
+class AdamWConfig(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("step", C.c_int32),
+                ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("state_bits", C.c_int32), ("grad_scale", C.c_void_p),
+                ("lr_device", C.c_void_p), ("step_device", C.c_void_p)]
 
 
 class Counters(C.Structure):
@@ -150,6 +170,13 @@ SIGNATURES = {
     "ob200_search_debug_phases": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p]),
     "ob200_search_debug_record": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
     "ob200_copy_to_host": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64]),
+    "ob200_launch_policy_loss_search": (C.c_int, [C.POINTER(PolicyRows), C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_void_p]),
+    "ob200_launch_policy_loss_clipped": (C.c_int, [C.POINTER(PolicyRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                                   C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float, C.c_void_p]),
+    "ob200_grad_norm_workspace_bytes": (C.c_int64, []),
+    "ob200_launch_grad_norm": (C.c_int, [C.POINTER(TrainTensor), C.c_int32, C.c_int32, C.c_float, C.c_void_p, C.c_void_p,
+                                         C.c_void_p]),
+    "ob200_launch_adamw": (C.c_int, [C.POINTER(TrainTensor), C.c_int32, C.POINTER(AdamWConfig), C.c_void_p]),
     "ob200_get_counters": (C.c_int, [C.POINTER(Counters)]),
     "ob200_reset_counters": (None, []),
 }
@@ -582,3 +609,225 @@ class Search:
             self.close()
         except Exception:
             pass
+
+
+# ---- training operators ---------------------------------------------------------------
+def _require(ok, text, *args):
+    if not ok:
+        raise Error(ERR_INVALID, text % args if args else text)
+
+
+def _train_dtype(t, what):
+    import torch
+    kinds = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+    _require(t.dtype in kinds, "%s: float32, bfloat16 or float16 is wanted, got %s", what, t.dtype)
+    return kinds[t.dtype]
+
+
+class _On:
+    """Makes a tensor's device the current one for a launch; gives the launch its current stream."""
+
+    def __init__(self, device):
+        import torch
+        _require(device.type == "cuda", "the tensors are not on a CUDA device (there is no CPU path)")
+        self.back = torch.cuda.current_device()
+        self.device, self.torch = device, torch
+
+    def __enter__(self):
+        if self.device.index != self.back:
+            self.torch.cuda.set_device(self.device)
+        return C.c_void_p(self.torch.cuda.current_stream().cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.device.index != self.back:
+            self.torch.cuda.set_device(self.back)
+
+
+def _matrix(t, what, n, A, device, dtype=None):
+    """Pitch of a matrix of n rows of A adjacent elements."""
+    _require(t.dim() == 2 and t.shape[0] == n and t.shape[1] == A, "%s: shape (%d, %d) is wanted, got %s", what, n, A, tuple(t.shape))
+    _require(t.device == device, "%s is on another device than the logits", what)
+    _require(dtype is None or t.dtype == dtype, "%s: %s is wanted, got %s", what, dtype, t.dtype)
+    _require(A == 1 or t.stride(1) == 1, "%s: the elements of a row have to be adjacent", what)
+    return t.stride(0) if n > 1 else max(t.stride(0), A)
+
+
+def _vector(t, what, n, device, dtype):
+    if t is None:
+        return None
+    _require(t.dtype == dtype and t.device == device and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1),
+             "%s: %d adjacent values of %s on the logits' device are wanted", what, n, dtype)
+    return t.data_ptr()
+
+
+def _policy_rows(logits, legal_bits, row_weight, out):
+    """The struct of both losses, and (loss, grad, stats)."""
+    import torch
+    _require(logits.dim() == 2 and logits.shape[1] > 0, "logits: a matrix of rows is wanted, got shape %s", tuple(logits.shape))
+    n, A = logits.shape
+    dtype, dev = _train_dtype(logits, "logits"), logits.device
+    if out is None:
+        out = (torch.empty(n, dtype=torch.float32, device=dev), torch.empty((n, A), dtype=logits.dtype, device=dev),
+               torch.empty((n, 4), dtype=torch.float32, device=dev))
+    loss, grad, stats = out
+    words = 0
+    if legal_bits is not None:
+        _require(legal_bits.dim() == 2 and legal_bits.shape[0] == n and legal_bits.dtype == torch.int32 and legal_bits.device == dev
+                 and legal_bits.is_contiguous(), "legal_bits: a contiguous int32 matrix [%d, words] on the logits' device is wanted", n)
+        words = legal_bits.shape[1]
+    if stats is not None:
+        _require(stats.dtype == torch.float32 and stats.device == dev and tuple(stats.shape) == (n, 4) and stats.is_contiguous(),
+                 "stats: a contiguous float32 matrix [%d, 4] on the logits' device is wanted", n)
+    pitch, grad_pitch = _matrix(logits, "logits", n, A, dev), _matrix(grad, "grad", n, A, dev, logits.dtype)
+    rows = PolicyRows(logits.data_ptr(), None if legal_bits is None else legal_bits.data_ptr(),
+                      _vector(row_weight, "row_weight", n, dev, torch.float32), grad.data_ptr(),
+                      _vector(loss, "loss", n, dev, torch.float32), None if stats is None else stats.data_ptr(),
+                      pitch, grad_pitch, n, A, words, dtype)
+    return rows, out
+
+
+def policy_loss_search(logits, target, legal_bits=None, row_weight=None, entropy_coef=0.0, out=None):
+    """Cross entropy of the policy with the search's visit distribution, row by row, and its gradient
+    (ob200_launch_policy_loss_search).  logits [n, A] float32 / bfloat16 / float16, target [n, A] int32 visit counts or
+    float32, legal_bits [n, words] int32 bit masks as DeviceTree holds them, row_weight [n] float32: the factor of each
+    row's loss, 0 for rows that only fill up a batch.  Returns (loss [n] float32, grad [n, A] of the logits' type,
+    stats [n, 4] float32: cross entropy, entropy, sum of the target, log-sum-exp); `out`: the three to write into (loss and
+    stats may be None, grad may be the logits).  With logits from autograd: torch.autograd.backward(logits, grad)."""
+    import torch
+    rows, out = _policy_rows(logits, legal_bits, row_weight, out)
+    kind = {torch.int32: TARGET_VISITS, torch.float32: TARGET_PROBS}.get(target.dtype)
+    _require(kind is not None, "target: int32 or float32 is wanted, got %s", target.dtype)
+    pitch = _matrix(target, "target", rows.n, rows.n_actions, logits.device)
+    with _On(logits.device) as stream:
+        check(lib().ob200_launch_policy_loss_search(C.byref(rows), target.data_ptr(), pitch, kind, entropy_coef, stream))
+    return out
+
+
+def policy_loss_clipped(logits, action, old_logp, advantage, legal_bits=None, ref_logits=None, row_weight=None, clip_low=0.2,
+                        clip_high=0.2, kl_coef=0.0, entropy_coef=0.0, out=None):
+    """Clipped-ratio policy loss with a KL term against a reference policy, row by row, and its gradient
+    (ob200_launch_policy_loss_clipped).  action [n] int32, old_logp and advantage [n] float32, ref_logits [n, A] of the
+    logits' type or None; the rest as policy_loss_search.  stats: log-probability of the action, ratio, KL, entropy."""
+    import torch
+    rows, out = _policy_rows(logits, legal_bits, row_weight, out)
+    dev, n = logits.device, rows.n
+    ref, ref_pitch = None, 0
+    if ref_logits is not None:
+        ref, ref_pitch = ref_logits.data_ptr(), _matrix(ref_logits, "ref_logits", n, rows.n_actions, dev, logits.dtype)
+    _require(action is not None and old_logp is not None and advantage is not None, "action, old_logp and advantage are wanted")
+    act, old, adv = (_vector(action, "action", n, dev, torch.int32), _vector(old_logp, "old_logp", n, dev, torch.float32),
+                     _vector(advantage, "advantage", n, dev, torch.float32))
+    with _On(dev) as stream:
+        check(lib().ob200_launch_policy_loss_clipped(C.byref(rows), act, old, adv, ref, ref_pitch, clip_low, clip_high, kl_coef,
+                                                     entropy_coef, stream))
+    return out
+
+
+def _same_kind(tensors, what):
+    """The OB200_DTYPE_* and device that all tensors of a list share; each has to be contiguous."""
+    first = tensors[0]
+    for i, t in enumerate(tensors):
+        _require(t.dtype == first.dtype and t.device == first.device, "%s %d: type or device differs from the first one's", what, i)
+        _require(t.is_contiguous(), "%s %d is not contiguous", what, i)
+    return _train_dtype(first, what), first.device
+
+
+class GradNorm:
+    """2-norm over a fixed list of gradients and the factor that clips it (ob200_launch_grad_norm).  run(max_norm) fills
+    and returns `out` (float32 [2] on the device: norm, factor); `clip` is the factor as AdamW.step takes it.  The plan
+    keeps the gradients and its workspace: one plan per stream that runs at the same time."""
+
+    def __init__(self, grads, out=None):
+        import torch
+        self.grads = list(grads)
+        _require(len(self.grads) > 0, "GradNorm: no gradients")
+        self.dtype, self.device = _same_kind(self.grads, "grad")
+        _require(self.device.type == "cuda", "the tensors are not on a CUDA device (there is no CPU path)")
+        self.out = torch.zeros(2, dtype=torch.float32, device=self.device) if out is None else out
+        _require(self.out.dtype == torch.float32 and self.out.device == self.device and tuple(self.out.shape) == (2,)
+                 and self.out.is_contiguous(), "GradNorm: out is float32 [2] on the gradients' device")
+        self.clip = self.out[1:]
+        self.workspace = torch.empty(int(lib().ob200_grad_norm_workspace_bytes()) // 8, dtype=torch.float64, device=self.device)
+        self.table = (TrainTensor * len(self.grads))()
+        for e, g in zip(self.table, self.grads):
+            e.grad, e.numel = g.data_ptr(), g.numel()
+
+    def run(self, max_norm=float("inf")):
+        with _On(self.device) as stream:
+            check(lib().ob200_launch_grad_norm(self.table, len(self.table), self.dtype, max_norm, self.workspace.data_ptr(),
+                                               self.out.data_ptr(), stream))
+        return self.out
+
+
+class AdamW:
+    """AdamW over a fixed list of weights and gradients, one launch a step (ob200_launch_adamw).
+
+    params, grads: contiguous tensors of one float type each on one device; the gradients' buffers are kept, so whatever
+    fills them has to write in place.  state_bits: 32, or 8 (e4m3 codes with a float32 scale per 256 elements).
+    weight_decay: a number, or one per tensor.  state: {"exp_avg": [...], "exp_avg_sq": [...]} and for 8 bits
+    {"exp_avg_scale": [...], "exp_avg_sq_scale": [...]} to go on from, zeros otherwise; it is `self.state`, updated in
+    place.  `self.steps` counts the steps made."""
+
+    BLOCK = 256
+
+    def __init__(self, params, grads, state_bits=32, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state=None):
+        import torch
+        self.params, self.grads = list(params), list(grads)
+        n = len(self.params)
+        _require(n > 0 and len(self.grads) == n, "AdamW: as many gradients as params are wanted, at least one")
+        _require(state_bits in (8, 32), "AdamW: state_bits is 8 or 32")
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+        _require(len(decay) == n, "AdamW: a weight decay for each param is wanted")
+        p_dtype, self.device = _same_kind(self.params, "param")
+        g_dtype, g_device = _same_kind(self.grads, "grad")
+        _require(self.device.type == "cuda", "the tensors are not on a CUDA device (there is no CPU path)")
+        _require(g_device == self.device, "AdamW: params and gradients are on different devices")
+        for i, (p, g) in enumerate(zip(self.params, self.grads)):
+            _require(p.numel() == g.numel(), "AdamW: param %d has %d elements, its gradient %d", i, p.numel(), g.numel())
+        held = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        keys = {"exp_avg": (held, 1), "exp_avg_sq": (held, 1)}
+        if state_bits == 8:
+            keys.update(exp_avg_scale=(torch.float32, self.BLOCK), exp_avg_sq_scale=(torch.float32, self.BLOCK))
+
+        def size(p, per):
+            return (p.numel() + per - 1) // per
+        if state is None:
+            state = {k: [torch.zeros(size(p, per), dtype=torch.uint8 if dt == torch.float8_e4m3fn else dt, device=self.device).view(dt)
+                         for p in self.params] for k, (dt, per) in keys.items()}
+        self.state = {k: list(state[k]) if k in state else None for k in keys}
+        for k, (dt, per) in keys.items():
+            _require(self.state[k] is not None and len(self.state[k]) == n, "AdamW: state %s: a tensor for each param is wanted", k)
+            for i, (t, p) in enumerate(zip(self.state[k], self.params)):
+                _require(t.dtype == dt and t.device == self.device and t.is_contiguous() and t.numel() == size(p, per),
+                         "AdamW: state %s %d: %d contiguous values of %s are wanted", k, i, size(p, per), dt)
+        self.table = (TrainTensor * n)()
+        for i, e in enumerate(self.table):
+            e.param, e.grad, e.numel, e.weight_decay = self.params[i].data_ptr(), self.grads[i].data_ptr(), self.params[i].numel(), decay[i]
+            for k in keys:
+                setattr(e, k, self.state[k][i].data_ptr())
+        self.cfg = AdamWConfig(beta1=betas[0], beta2=betas[1], eps=eps, param_dtype=p_dtype, grad_dtype=g_dtype, state_bits=state_bits)
+        self.steps = 0
+
+    def _scalar(self, t, what, dtype):
+        _require(t.dtype == dtype and t.device == self.device and t.numel() == 1, "AdamW: %s is one %s on the weights' device", what, dtype)
+        return t.data_ptr()
+
+    def step(self, lr, step=None, grad_scale=None):
+        """One step.  lr: a number, or a float32 scalar on the device; step: 1 for the first one (default: counted here), or an
+        int32 scalar on the device - for captured graphs; grad_scale: a float32 scalar on the device that multiplies every
+        gradient (GradNorm.clip), and leaves the step out when it is not finite."""
+        import torch
+        c = self.cfg
+        c.grad_scale = None if grad_scale is None else self._scalar(grad_scale, "grad_scale", torch.float32)
+        if torch.is_tensor(lr):
+            c.lr, c.lr_device = 0.0, self._scalar(lr, "lr", torch.float32)
+        else:
+            c.lr, c.lr_device = lr, None
+        if torch.is_tensor(step):
+            c.step, c.step_device = 0, self._scalar(step, "step", torch.int32)
+        else:
+            c.step, c.step_device = self.steps + 1 if step is None else step, None
+        with _On(self.device) as stream:
+            check(lib().ob200_launch_adamw(self.table, len(self.table), C.byref(c), stream))
+        if not torch.is_tensor(step):
+            self.steps = c.step
