@@ -670,13 +670,19 @@ int ob200_copy_to_host(void* dst_host, const void* src_device, int64_t bytes);
 #define OB200_DTYPE_F32 2       /* policy rows, gradients and weights only       */
 
 /* Rows of policy logits, one per position, with what every policy loss writes.
- * An action counts as legal when its bit is set (legal_bits NULL: all are) and
- * its logit is not -inf; the policy is the softmax over the legal actions, and
- * what stands at other places (infinities and NaN included) is not looked at.
+ * An action is legal when its bit is set (legal_bits NULL: all are); the policy
+ * is the softmax over the legal actions, and what stands at other places
+ * (infinities and NaN included) does not matter.  A logit of -inf is a
+ * probability of 0; in sums over differences of logits (H, KL, cross entropy)
+ * those below -1e30 count as -1e30.
  * A row is left out - loss, statistics and gradient are 0 - when its weight is 0
- * (it is then not read), when it has no legal action, or for the reason its
- * loss names.  A NaN or +inf logit of a legal action makes its row's results
- * NaN.  Columns from n_actions to the pitch are neither read nor written. */
+ * (its logits are then not read), when no legal action has a logit above -inf, or
+ * for the reason its loss names.  A NaN or +inf logit of a legal action makes its
+ * row's results NaN.  Columns from n_actions to the pitch are not written, and
+ * what they hold does not matter.
+ * Matrices whose rows start at the same place within 16 bytes of each other's
+ * (all contiguous ones from the usual allocators) are read and written 16 bytes
+ * at a time, others element by element. */
 typedef struct ob200_policy_rows {
     const void* logits;         /* [n][logits_pitch] of dtype                     */
     const uint32_t* legal_bits; /* [n][mask_words] as ob200_tree_view, or NULL    */
@@ -715,9 +721,10 @@ int ob200_launch_policy_loss_search(const ob200_policy_rows* rows, const void* t
  *   stats = (log p[action], r, KL, H).
  * The gradient of the first term is that of r * advantage where it is not the
  * larger one, 0 elsewhere; an advantage of 0 contributes 0 whatever r is.
- * ref_logits may be NULL (KL = 0; kl_coef must then be 0).  A row whose action is
- * outside [0, n_actions) or not legal is left out.  KL is not finite where q gives
- * no probability to an action that p gives some. */
+ * ref_logits may be NULL (KL = 0; kl_coef must then be 0).  KL becomes very large,
+ * not infinite, where q gives no probability to an action that p gives some (and
+ * infinite where q gives none to any).  A row whose action is outside
+ * [0, n_actions) or not legal is left out. */
 int ob200_launch_policy_loss_clipped(const ob200_policy_rows* rows, const int32_t* action, const float* old_logp,
                                      const float* advantage, const void* ref_logits, int64_t ref_pitch,
                                      float clip_low, float clip_high, float kl_coef, float entropy_coef,

@@ -283,6 +283,7 @@ def test_lowest_values_and_infinities(api, dt, A):
     z[3, 1:] = -float("inf")             # one action
     z[4, 3] = float("nan")               # a NaN counts
     t = torch.ones((5, A))
+    t[3, 1:] = 0
     loss, grad, stats = api.policy_loss_search(z.cuda(), t.cuda())
     torch.cuda.synchronize()
     grad, stats = grad.double().cpu(), stats.double().cpu()
