@@ -10,13 +10,16 @@
 //   clipped term: d/dz_j = k ([j = action] - p_j),  k = -advantage r or 0
 // so a gradient is p_j (k0 + kz d_j + kd (d_j - d'_j)) plus a term of the action or of the target.
 //
-// A team - a warp, a CTA, or the CTAs of a cluster - works on a row that bulk copies have brought into shared memory while
-// it was busy with the row before: once for the maximum (where actions that do not count are replaced by -inf, so that the
-// other passes ask no mask), once for the sums, once for the gradient, which leaves in 16-byte stores.  Every matrix is
-// read from memory once and the gradient written once.  What bounds the kernel next to memory is instructions: at
-// 6.5 TB/s an SM has 33 thread instructions for an action of 16-bit logits with a reference row (6 bytes), 66 in fp32;
-// hence the packed arithmetic (two fp32 an instruction), the packed 16-bit maximum, and few threads a row, each with many
-// actions, over which the joining of sums is spread.
+// Rows are worked on in shared memory, where bulk copies have brought them while the rows before were worked on: once for
+// the maximum (where actions that do not count are replaced by a lowest value, so that the other passes ask no mask), once
+// for the sums, once for the gradient, which leaves in 16-byte stores.  Every matrix is read from memory once and the
+// gradient written once.  Next to memory, instructions are what bounds it: at 6.5 TB/s an SM has 33 thread instructions
+// for an action of 16-bit logits with a reference row (6 bytes), 66 in fp32.  Hence the packed arithmetic (two fp32 an
+// instruction), the packed 16-bit maximum, and few threads a row, each with many actions:
+//   policy_warp_rows_kernel   short rows: 8, 16 or 32 lanes a row, so that what a row costs besides its actions is paid
+//                             once for up to four of them
+//   policy_cta_rows_kernel    the others: a CTA or the CTAs of a cluster a row, one warp copying ahead, one joining sums
+//   policy_long_rows_kernel   rows beyond the shared memory of eight CTAs, three times through device memory
 #pragma once
 #include "common.h"
 #include "internal.h"
@@ -81,13 +84,19 @@ __device__ __forceinline__ float warp_max_nan(float v) {
     asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xFFFFFFFF;" : "=f"(y) : "f"(v));
     return y;
 }
-__device__ __forceinline__ float warp_sum(float v) {
+// Over the LANES lanes of a team.
+template <int LANES = 32>
+__device__ __forceinline__ float team_sum(float v) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     return v;
 }
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+template <int LANES = 32>
+__device__ __forceinline__ float team_max_nan(float v) {
+    if (LANES == 32) return warp_max_nan(v);
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+    return v;
 }
 
 // Two fp32 in a register pair.
@@ -118,11 +127,6 @@ __device__ __forceinline__ f32x2 ex2_2(f32x2 v) {
     halves(v, a, b);
     return pair(ex2(a), ex2(b));
 }
-__device__ __forceinline__ f32x2 floor2(f32x2 v) {            // not below kLow
-    float a, b;
-    halves(v, a, b);
-    return pair(fmaxf(a, kLow), fmaxf(b, kLow));
-}
 __device__ __forceinline__ float sum2(f32x2 v) {
     float a, b;
     halves(v, a, b);
@@ -130,10 +134,12 @@ __device__ __forceinline__ float sum2(f32x2 v) {
 }
 
 // ---- 16 bytes of a row ------------------------------------------------------------
-template <typename T> struct Bits;                              // per type: -inf in every element of a word
-template <> struct Bits<float> { static constexpr uint32_t kNinf = 0xFF800000u; };
-template <> struct Bits<__nv_bfloat16> { static constexpr uint32_t kNinf = 0xFF80FF80u; };
-template <> struct Bits<__half> { static constexpr uint32_t kNinf = 0xFC00FC00u; };
+// The value that stands for logits that do not count, and for those below it: in every element of a word, and as fp32.
+// A row whose largest logit is below half of it is worked on separately (careful_row).
+template <typename T> struct Lowest;
+template <> struct Lowest<float> { static constexpr uint32_t kWord = 0xF149F2CAu; static constexpr float kValue = -1e30f; };
+template <> struct Lowest<__nv_bfloat16> { static constexpr uint32_t kWord = 0xF149F149u; static constexpr float kValue = -9.95e29f; };
+template <> struct Lowest<__half> { static constexpr uint32_t kWord = 0xFBFFFBFFu; static constexpr float kValue = -65504.f; };
 
 // Elements 2i and 2i + 1 of a vector of T as fp32.
 template <typename T>
@@ -202,33 +208,26 @@ struct RowOut { float loss; float4 stats; };
 // False when the row is left out.
 template <int KIND>
 __device__ __forceinline__ bool row_result(const PolicyRows& r, const Sums& q, float w, float old_logp, float adv, RowGrad* g, RowOut* o) {
-    if (q.m == -kInf) return false;
     const float l2s = lg2(q.s), ls = l2s * kLn2, inv_s = __fdividef(1.f, q.s), mean = q.t * inv_s, H = ls - mean;
-    g->M = q.m; g->C = q.c == -kInf ? 0.f : q.c; g->lp = -l2s;
+    g->M = q.m; g->C = q.c; g->lp = -l2s;
     g->kz = w * r.entropy; g->kd = 0.f; g->ka = 0.f; g->kt = 0.f;
     if (KIND == kSearch) {
-        if (!(q.b != 0.f)) return false;
         const float inv_T = 1.f / q.b, ce = fmaf(-q.a, inv_T, ls);
         g->k0 = w * (1.f - r.entropy * mean);
         g->kt = w * inv_T;
         o->loss = w * (ce - r.entropy * H);
         o->stats = make_float4(ce, H, q.b, q.m + ls);
-        return true;
+        return q.b != 0.f;
     }
-    if (q.za == -kInf) return false;
-    const float logp = max_nan(q.za - q.m, kLow) - ls;
+    const float logp = (q.za - q.m) - ls;
     const float ratio = ex2((logp - old_logp) * kLog2e);
-    float surrogate = 0.f, k = 0.f;
-    if (adv != 0.f) {
-        const float open = ratio * adv, held = fminf(fmaxf(ratio, r.lo), r.hi) * adv;
-        surrogate = open <= held ? open : held;
-        k = open <= held ? -open : 0.f;
-        if (open != open) surrogate = k = open;
-    }
+    const float open = ratio * adv, held = fminf(fmaxf(ratio, r.lo), r.hi) * adv;
+    const bool free = open <= held || open != open, none = adv == 0.f;
+    const float surrogate = none ? 0.f : free ? open : held, k = none || !free ? 0.f : -open;
     float kl = 0.f, ud = 0.f;
     if (KIND == kClippedRef) {
         ud = q.a * inv_s;
-        kl = q.b == 0.f ? kInf : ud - (l2s - lg2(q.b)) * kLn2;       // 0: q gives nothing to any legal action
+        kl = ud - (l2s - lg2(q.b)) * kLn2;
         if (kl != kl) ud = kl;
     }
     g->k0 = w * (-k - r.kl * ud - r.entropy * mean);
@@ -236,455 +235,66 @@ __device__ __forceinline__ bool row_result(const PolicyRows& r, const Sums& q, f
     g->ka = w * k;
     o->loss = w * (-surrogate + r.kl * kl - r.entropy * H);
     o->stats = make_float4(logp, ratio, kl, H);
-    return true;
+    return q.za != -kInf;
+}
+
+__device__ __forceinline__ void put_out(const PolicyRows& r, long long row, bool live, const RowOut& o) {
+    if (r.loss) r.loss[row] = live ? o.loss : 0.f;
+    if (r.stats) r.stats[row] = live ? o.stats : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 __device__ __forceinline__ bool legal(const uint32_t* bits, int j) { return !bits || (bits[j >> 5] >> (j & 31)) & 1u; }
 __device__ __forceinline__ float target_f32(uint32_t raw, int visits) { return visits ? (float)(int)raw : __uint_as_float(raw); }
 
-// ---- rows in shared memory ------------------------------------------------------------
-// How rows lie there.  A slot holds a team's part of a row: its scalars (16 bytes), vectors of 16 bytes of logits, what
-// belongs to them of the second matrix, and the words of the mask.
-struct RowShape {
-    int seg;                            // vectors a CTA holds of a row
-    int x_at, mask_at, slot_bytes;      // offsets in a slot, its size
-    int slots, team_bytes;              // slots in turn; bytes of a team's slots and barriers
-    int* error;
-};
-
-__device__ __forceinline__ void copy_word_async(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-// WARP: a warp per row.  Else the CTA, or the cluster's CTAs, work on a row together.  ALIKE: the rows of the matrices start
-// at the same element of 16 bytes, so vectors are copied and stored whole; else element by element.
-template <typename T, int KIND, bool WARP, bool ALIKE>
-__global__ void __launch_bounds__(WARP ? 256 : 512, 2)
-policy_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {
-    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float top_of[2][16][2];
-    __shared__ float part[2][128][8];            // what the warps of the team found, by turns
-    __shared__ int abort_flag;
-    uint32_t cta = 0, ctas = 1;
-    if (!WARP) {
-        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
-        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-    }
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
-    const int tid = WARP ? lane : threadIdx.x, team = WARP ? 32 : blockDim.x;
-    const long long first = WARP ? (long long)blockIdx.x * warps + warp : blockIdx.x / ctas;
-    const long long step = WARP ? (long long)gridDim.x * warps : gridDim.x / ctas;
-    uint8_t* const mine = smem + (WARP ? warp * sh.team_bytes : 0);
-    const uint32_t mine_s = ptx::smem_u32(mine), bars = mine_s + sh.slots * sh.slot_bytes;
-    if (ALIKE && tid == 0)
-        for (int s = 0; s < sh.slots; ++s) ptx::mbar_init(bars + 8 * s, r.bits ? 1 + team : 1);
-    if (threadIdx.x == 0) abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncthreads();
-    // the cluster's CTAs write into each other's shared memory: all of them have to be there
-    if (!WARP && ctas > 1) cluster_barrier();
-
-    const int v0 = (int)cta * sh.seg;
-    const uintptr_t z0 = (uintptr_t)r.z, x0 = (uintptr_t)r.x;
-    const uintptr_t z1 = z0 + ((r.n - 1) * r.z_pitch + r.A) * sizeof(T), x1 = x0 + ((r.n - 1) * r.x_pitch + r.A) * XB;
-    // Where row q lies: its first element's place in the first vector, vectors, this CTA's; whether the outer vectors
-    // reach beyond the matrices (the others' ends hold what stands beside the row, which the first pass replaces).
-    struct Place { int head, vecs, v1; bool first_out, last_out; };
-    auto place_of = [&](long long q) {
-        Place p;
-        p.head = ALIKE ? (int)((r.phase + q * r.z_pitch) % V) : 0;
-        p.vecs = (p.head + r.A + V - 1) / V;
-        p.v1 = min(p.vecs, v0 + sh.seg);
-        const uintptr_t za = z0 + (q * r.z_pitch - p.head) * sizeof(T), xa = x0 + (q * r.x_pitch - p.head) * XB;
-        p.first_out = za < z0 || (KIND != kClipped && xa < x0);
-        p.last_out = za + p.vecs * 16 > z1 || (KIND != kClipped && xa + (uintptr_t)p.vecs * XV > x1);
-        return p;
-    };
-    // Row q into slot s, asynchronously.  scalars: thread 0's.
-    auto fill = [&](long long q, int s, float4 scalars) {
-        const uint32_t slot = mine_s + s * sh.slot_bytes, bar = bars + 8 * s;
-        const Place p = place_of(q);
-        if (r.bits) {
-            const int w0 = max(v0 * V - p.head, 0) >> 5, w1 = (min(p.v1 * V - p.head, r.A) - 1) >> 5;
-            const uint32_t* from = r.bits + q * r.mask_words;
-            for (int i = w0 + tid; i <= w1; i += team) copy_word_async(slot + sh.mask_at + 4 * (i - w0), from + i);
-            arrive_after_copies(bar);
-        }
-        if (tid == 0) {
-            *(float4*)(mine + s * sh.slot_bytes) = scalars;
-            int lo = v0, hi = p.v1;
-            if (lo == 0 && p.first_out) lo = 1;
-            if (hi == p.vecs && p.last_out) --hi;
-            if (scalars.x != 0.f && hi > lo) {
-                const int n = hi - lo;
-                const uintptr_t za = z0 + (q * r.z_pitch - p.head) * sizeof(T), xa = x0 + (q * r.x_pitch - p.head) * XB;
-                ptx::mbar_arrive_expect_tx(bar, n * (KIND == kClipped ? 16 : 16 + XV));
-                ptx::bulk_g2s(slot + 16 + (lo - v0) * 16, (const void*)(za + (uintptr_t)lo * 16), n * 16, bar);
-                if (KIND != kClipped) ptx::bulk_g2s(slot + sh.x_at + (lo - v0) * XV, (const void*)(xa + (uintptr_t)lo * XV), n * XV, bar);
-            } else {
-                ptx::mbar_arrive(bar);
-            }
-        }
-    };
-    auto scalars_of = [&](long long q) {
-        float4 v = make_float4(1.f, 0.f, 0.f, 0.f);
-        if (q >= r.n) return v;
-        if (r.weight) v.x = r.weight[q];
-        if (KIND != kSearch) { v.y = r.old_logp[q]; v.z = r.advantage[q]; v.w = __int_as_float(r.action[q]); }
-        return v;
-    };
-    float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);      // scalars of the next row to be copied
-    if (ALIKE) {
-        for (int s = 0; s < sh.slots; ++s)
-            if (first + s * step < r.n) fill(first + s * step, s, scalars_of(first + s * step));
-        if (tid == 0) ahead = scalars_of(first + sh.slots * step);
-    }
-
-    int slot = 0, turn = 0, part_turn = 0, last_slot = -1;
-    uint32_t parity = 0;
-    for (long long row = first; row < r.n; row += step) {
-        uint8_t* const at = mine + slot * sh.slot_bytes;
-        uint8_t *const zs = at + 16, *const xs = at + sh.x_at;
-        const uint32_t* const ms = (const uint32_t*)(at + sh.mask_at);
-        const Place p = place_of(row);
-        const int mask_first = max(v0 * V - p.head, 0) >> 5;
-        float4 scalars;
-        if (ALIKE) {
-            if (!ptx::mbar_wait(bars + 8 * slot, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
-            scalars = *(const float4*)at;
-        } else {
-            scalars = scalars_of(row);
-            if (scalars.x != 0.f) {
-                const int j1 = min(p.v1 * V, r.A);
-                const T* z = (const T*)r.z + row * r.z_pitch;
-                for (int j = v0 * V + tid; j < j1; j += team) {
-                    ((T*)zs)[j - v0 * V] = z[j];
-                    if (KIND == kSearch) ((uint32_t*)xs)[j - v0 * V] = ((const uint32_t*)r.x)[row * r.x_pitch + j];
-                    if (KIND == kClippedRef) ((T*)xs)[j - v0 * V] = ((const T*)r.x)[row * r.x_pitch + j];
-                }
-                if (r.bits)
-                    for (int i = mask_first + tid; i <= (j1 - 1) >> 5; i += team) ((uint32_t*)ms)[i - mask_first] = r.bits[row * r.mask_words + i];
-            }
-            if (WARP) __syncwarp(); else __syncthreads();
-        }
-        const float w = scalars.x;
-        const int act = KIND == kSearch ? -1 : __float_as_int(scalars.w);
-        const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;     // the action's element of the row
-        bool live = w != 0.f;
-        RowGrad g;
-        RowOut out{0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-
-        // the maximum; what does not count becomes -inf (a target 0), visit counts become fp32
-        uint32_t top_z = Bits<T>::kNinf, top_x = Bits<T>::kNinf;
-        if (live) {
-            const int edge_first = p.head ? 0 : -1, edge_last = (p.head + r.A) % V ? p.vecs - 1 : -1;
-            for (int v = v0 + tid; v < p.v1; v += team) {
-                uint8_t *zp = zs + (v - v0) * 16, *xp = xs + (v - v0) * XV;
-                uint32_t z[4], x[XV / 4];
-                load16(zp, z);
-                const bool edge = v == edge_first || v == edge_last;
-                if (KIND == kClippedRef || (KIND == kSearch && (r.bits || r.visits || edge)))
-#pragma unroll
-                    for (int i = 0; i < XV / 16; ++i) load16(xp + 16 * i, x + 4 * i);
-                if (r.bits || edge) {
-                    const int j = v * V - p.head;                   // the first element's action; below 0 in the first vector
-                    uint32_t on = ~0u;
-                    if (r.bits) {
-                        const int i = (j >> 5) - mask_first, most = (r.A - 1) >> 5;
-                        const uint32_t lo = j < 0 ? 0u : ms[i], hi = (j & 31) + V > 32 && (j >> 5) < most ? ms[i + 1] : 0u;
-                        on = __funnelshift_r(lo, hi, j & 31);
-                    }
-                    if (j < 0) on &= ~0u << -j;
-                    if (j + V > r.A) on &= ~(~0u << (r.A - j));
-                    if (ALIKE && ((v == 0 && p.first_out) || (v == p.vecs - 1 && p.last_out))) {
-                        // not copied: it reaches beyond the matrix
-                        for (int i = 0; i < V; ++i)
-                            if (j + i >= 0 && j + i < r.A) {
-                                ((T*)zp)[i] = ((const T*)r.z)[row * r.z_pitch + j + i];
-                                if (KIND == kSearch) ((uint32_t*)xp)[i] = ((const uint32_t*)r.x)[row * r.x_pitch + j + i];
-                                if (KIND == kClippedRef) ((T*)xp)[i] = ((const T*)r.x)[row * r.x_pitch + j + i];
-                            }
-                        load16(zp, z);
-                        if (KIND != kClipped)
-#pragma unroll
-                            for (int i = 0; i < XV / 16; ++i) load16(xp + 16 * i, x + 4 * i);
-                    }
-                    uint32_t m[4];
-                    word_masks<T>(on, m);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        z[i] = (z[i] & m[i]) | (Bits<T>::kNinf & ~m[i]);
-                        if (KIND == kClippedRef) x[i] = (x[i] & m[i]) | (Bits<T>::kNinf & ~m[i]);
-                    }
-                    store16(zp, z);
-                    if (KIND == kClippedRef) store16(xp, x);
-                    if (KIND == kSearch)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) x[i] = (on >> i) & 1u ? x[i] : 0u;
-                }
-                if (KIND == kSearch && (r.bits || r.visits || edge)) {
-                    if (r.visits)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) x[i] = __float_as_uint((float)(int)x[i]);
-#pragma unroll
-                    for (int i = 0; i < XV / 16; ++i) store16(xp + 16 * i, x + 4 * i);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    top_z = word_max<T>(top_z, z[i]);
-                    if (KIND == kClippedRef) top_x = word_max<T>(top_x, x[i]);
-                }
-            }
-        }
-        Sums q;
-        q.m = warp_max_nan(word_top<T>(top_z));
-        q.c = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : -kInf;
-        q.s = q.t = q.a = q.b = 0.f;
-        q.za = -kInf;
-        if (WARP) {
-            __syncwarp();
-        } else {
-            if (lane == 0) { top_of[turn][warp][0] = q.m; top_of[turn][warp][1] = q.c; }
-            __syncthreads();
-            if (ALIKE && last_slot >= 0) {
-                // every thread is done with the row before: its slot takes the next one
-                const long long next = row + (sh.slots - 1) * step;
-                if (next < r.n) {
-                    fill(next, last_slot, ahead);
-                    if (tid == 0) ahead = scalars_of(next + step);
-                }
-            }
-            const int i = lane < warps ? lane : 0;
-            q.m = warp_max_nan(top_of[turn][i][0]);
-            if (KIND == kClippedRef) q.c = warp_max_nan(top_of[turn][i][1]);
-        }
-        if (live && act_e >= 0 && act_e / V >= v0 && act_e / V < p.v1 && (!r.bits || (ms[(act >> 5) - mask_first] >> (act & 31)) & 1u)) {
-            const float v = to_f32(((const T*)zs)[act_e - v0 * V]);
-            q.za = v == -kInf ? -3.4e38f : v;
-        }
-
-        // the sums
-        if (live && q.m != -kInf) {
-            const f32x2 M = pair(-q.m, -q.m), C = q.c == -kInf ? pair(0.f, 0.f) : pair(-q.c, -q.c), L = pair(kLog2e, kLog2e), minus = pair(-1.f, -1.f);
-            f32x2 s = 0, t = 0, a = 0, b = 0;
-#pragma unroll 2
-            for (int v = v0 + tid; v < p.v1; v += team) {
-                uint32_t z[4], x[XV / 4];
-                load16(zs + (v - v0) * 16, z);
-                if (KIND != kClipped)
-#pragma unroll
-                    for (int i = 0; i < XV / 16; ++i) load16(xs + (v - v0) * XV + 16 * i, x + 4 * i);
-#pragma unroll
-                for (int i = 0; i < V / 2; ++i) {
-                    const f32x2 d = add2(elements<T>(z, i), M), e = ex2_2(mul2(d, L)), dl = floor2(d);
-                    s = add2(s, e);
-                    t = fma2(e, dl, t);
-                    if (KIND == kSearch) {
-                        const f32x2 y = elements<float>(x, i);
-                        a = fma2(y, dl, a);
-                        b = add2(b, y);
-                    }
-                    if (KIND == kClippedRef) {
-                        const f32x2 c = add2(elements<T>(x, i), C);
-                        b = add2(b, ex2_2(mul2(c, L)));
-                        a = fma2(e, fma2(floor2(c), minus, dl), a);
-                    }
-                }
-            }
-            q.s = sum2(s); q.t = sum2(t); q.a = sum2(a); q.b = sum2(b);
-        }
-        if (live) {                              // the same in the whole team
-            q.s = warp_sum(q.s);
-            q.t = warp_sum(q.t);
-            if (KIND != kClipped) { q.a = warp_sum(q.a); q.b = warp_sum(q.b); }
-        }
-        if (!WARP && live) {
-            // every warp of the team leaves its sums with every CTA, and each warp joins them all, a lane an entry
-            float (*to)[8] = part[part_turn];
-            part_turn ^= 1;                      // only where a barrier follows: the other CTAs may still read the last ones
-            if (lane < (int)ctas) {
-                const uint32_t here = ptx::smem_u32(to[cta * warps + warp]);
-                uint32_t there;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(lane));
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(q.m), "f"(q.c), "f"(q.s), "f"(q.t) : "memory");
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + 16), "f"(q.a), "f"(q.b), "f"(q.za), "f"(0.f) : "memory");
-            }
-            if (ctas == 1) __syncthreads();
-            else cluster_barrier();
-            const int parts = (int)ctas * warps;
-            float M = -kInf, C = -kInf;
-            if (ctas == 1) {
-                M = q.m; C = q.c;
-            } else {
-                for (int i = lane; i < parts; i += 32) { M = max_nan(M, to[i][0]); C = max_nan(C, to[i][1]); }
-                M = warp_max_nan(M);
-                C = warp_max_nan(C);
-            }
-            q.s = q.t = q.a = q.b = 0.f;
-            for (int i = lane; i < parts; i += 32) {
-                float4 lo = *(const float4*)to[i];
-                const float4 hi = *(const float4*)(to[i] + 4);
-                if (ctas > 1) {
-                    // a CTA's sums are relative to its own maxima
-                    const float d = lo.x == -kInf ? 0.f : lo.x - M, c = lo.y == -kInf ? 0.f : lo.y - C;
-                    const float f = lo.x == -kInf ? 0.f : ex2(d * kLog2e);
-                    lo.z *= f;
-                    lo.w = fmaf(d, lo.z, lo.w * f);
-                    if (KIND == kSearch) q.a += fmaf(d, hi.y, hi.x);
-                    if (KIND == kClippedRef) { q.a += fmaf(d - c, lo.z, hi.x * f); q.b = fmaf(hi.y, lo.y == -kInf ? 0.f : ex2(c * kLog2e), q.b); }
-                } else {
-                    q.a += hi.x;
-                    if (KIND == kClippedRef) q.b += hi.y;
-                }
-                if (KIND == kSearch) q.b += hi.y;
-                q.s += lo.z;
-                q.t += lo.w;
-                q.za = max_nan(q.za, hi.z);
-            }
-            q.s = warp_sum(q.s);
-            q.t = warp_sum(q.t);
-            if (KIND != kClipped) { q.a = warp_sum(q.a); q.b = warp_sum(q.b); }
-            if (KIND != kSearch) q.za = warp_max_nan(q.za);
-            q.m = M; q.c = C;
-        }
-        turn ^= 1;
-        live = live && row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out);
-        if (tid == 0 && cta == 0) {
-            if (r.loss) r.loss[row] = out.loss;
-            if (r.stats) r.stats[row] = out.stats;
-        }
-
-        // the gradient
-        T* grad = (T*)r.grad + row * r.g_pitch - p.head;
-        const f32x2 M = pair(-g.M, -g.M), C = pair(-g.C, -g.C), L = pair(kLog2e, kLog2e), minus = pair(-1.f, -1.f);
-        const f32x2 lp = pair(g.lp, g.lp), k0 = pair(g.k0, g.k0), kz = pair(g.kz, g.kz), kd = pair(g.kd, g.kd), kt = pair(-g.kt, -g.kt);
-#pragma unroll 2
-        for (int v = v0 + tid; v < p.v1; v += team) {
-            uint32_t z[4] = {0, 0, 0, 0}, x[XV / 4];
-            float o[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = 0.f;
-            if (live) {
-                load16(zs + (v - v0) * 16, z);
-                if (KIND != kClipped)
-#pragma unroll
-                    for (int i = 0; i < XV / 16; ++i) load16(xs + (v - v0) * XV + 16 * i, x + 4 * i);
-#pragma unroll
-                for (int i = 0; i < V / 2; ++i) {
-                    const f32x2 d = add2(elements<T>(z, i), M), pr = ex2_2(fma2(d, L, lp)), dl = floor2(d);
-                    f32x2 y = fma2(kz, dl, k0);
-                    if (KIND == kClippedRef) y = fma2(kd, fma2(floor2(add2(elements<T>(x, i), C)), minus, dl), y);
-                    y = mul2(y, pr);
-                    if (KIND == kSearch) y = fma2(kt, elements<float>(x, i), y);
-                    halves(y, o[2 * i], o[2 * i + 1]);
-                }
-                if (KIND != kSearch && (unsigned)act_e - (unsigned)(v * V) < (unsigned)V)
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (act_e == v * V + i) o[i] += g.ka;
-            }
-            if (sizeof(T) == 4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = __float_as_uint(o[i % V]);
-            else
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = pack2<T>(o[(2 * i) % V], o[(2 * i + 1) % V]);
-            if (ALIKE) {
-                const int e = v * V;
-                if (e >= p.head && e + V <= p.head + r.A) {
-                    *(uint4*)(grad + e) = make_uint4(z[0], z[1], z[2], z[3]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (e + i >= p.head && e + i < p.head + r.A) grad[e + i] = from_f32<T>(o[i]);
-                }
-            } else {
-                store16(zs + (v - v0) * 16, z);
-            }
-        }
-        // the slot's next copy comes behind what was read and written here
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (!ALIKE) {
-            if (WARP) __syncwarp(); else __syncthreads();
-            const int j1 = min(p.v1 * V, r.A);
-            for (int j = v0 * V + tid; j < j1; j += team) grad[j] = ((const T*)zs)[j - v0 * V];
-            if (WARP) __syncwarp(); else __syncthreads();
-        } else if (WARP) {
-            __syncwarp();
-            const long long next = row + sh.slots * step;
-            if (next < r.n) {
-                fill(next, slot, ahead);
-                if (tid == 0) ahead = scalars_of(next + step);
-            }
-        }
-        last_slot = slot;
-        if (++slot == sh.slots) { slot = 0; parity ^= 1; }
-    }
-    if (ALIKE && abort_flag) {                   // a wait ran out: what is still in flight is waited for once more, within the same limit
-        int none = 0;
-        for (int s = 0; s < sh.slots; ++s) ptx::mbar_wait(bars + 8 * s, s >= slot ? parity : parity ^ 1, &none);
-    }
-    // and none may leave while another may still write
-    if (!WARP && ctas > 1) cluster_barrier();
-}
-
-// ---- rows of any length -----------------------------------------------------------
-// Rows too long for the shared memory of eight CTAs (from some 200,000 actions on): a CTA goes over its row in device
-// memory three times.
-template <typename T, int KIND>
-__global__ void __launch_bounds__(512)
-policy_long_rows_kernel(const __grid_constant__ PolicyRows r) {
-    const long long row = blockIdx.x;
+// ---- a row straight from device memory ---------------------------------------------------
+// `threads` threads (a warp, or a CTA of 512) go over a row three times; join(v, is_max) joins a value over them.
+template <typename T, int KIND, typename Join>
+__device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, int tid, int threads, Join join) {
     const T* z = (const T*)r.z + row * r.z_pitch;
     const uint8_t* x = (const uint8_t*)r.x + row * r.x_pitch * (KIND == kSearch ? 4 : sizeof(T));
     T* grad = (T*)r.grad + row * r.g_pitch;
     const uint32_t* bits = r.bits ? r.bits + row * r.mask_words : nullptr;
     const float w = r.weight ? r.weight[row] : 1.f;
-    const int act = KIND == kSearch ? -1 : r.action[row], lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int act = KIND == kSearch ? -1 : r.action[row];
     auto second = [&](int j) { return KIND == kSearch ? target_f32(((const uint32_t*)x)[j], r.visits) : KIND == kClippedRef ? to_f32(((const T*)x)[j]) : 0.f; };
-    __shared__ float part[2][16][8];
-    bool live = w != 0.f;
     Sums q{-kInf, -kInf, 0.f, 0.f, 0.f, 0.f, -kInf};
+    bool live = w != 0.f;
+    if (live && bits) {                          // most rows that come here have no legal action
+        float some = 0.f;
+        for (int i = tid; i < (r.A + 31) / 32; i += threads)
+            if (bits[i] & (i == r.A / 32 ? ~(~0u << (r.A & 31)) : ~0u)) some = 1.f;
+        live = join(some, true) != 0.f;
+    }
     if (live)
-        for (int j = threadIdx.x; j < r.A; j += 512)
+        for (int j = tid; j < r.A; j += threads)
             if (legal(bits, j)) {
                 const float v = to_f32(z[j]);
                 q.m = max_nan(q.m, v);
                 if (KIND == kClippedRef) q.c = max_nan(q.c, second(j));
                 if (KIND != kSearch && j == act) q.za = v == -kInf ? -3.4e38f : v;
             }
-    q.m = warp_max_nan(q.m); q.c = warp_max_nan(q.c); q.za = warp_max_nan(q.za);
-    if (lane == 0) { part[0][warp][0] = q.m; part[0][warp][1] = q.c; part[0][warp][2] = q.za; }
-    __syncthreads();
-    q.m = warp_max_nan(part[0][lane % 16][0]); q.c = warp_max_nan(part[0][lane % 16][1]); q.za = warp_max_nan(part[0][lane % 16][2]);
-    const float C = q.c == -kInf ? 0.f : q.c;
-    live = live && q.m != -kInf;                 // the same in the whole CTA
+    q.m = join(q.m, true);
+    if (KIND == kClippedRef) q.c = join(q.c, true);
+    if (KIND != kSearch) q.za = join(q.za, true);
+    live = live && q.m != -kInf;
+    if (KIND != kClippedRef || q.c == -kInf) q.c = 0.f;
     if (live)
-        for (int j = threadIdx.x; j < r.A; j += 512)
+        for (int j = tid; j < r.A; j += threads)
             if (legal(bits, j)) {
                 const float d = to_f32(z[j]) - q.m, e = ex2(d * kLog2e), dl = fmaxf(d, kLow), y = second(j);
                 q.s += e;
                 q.t = fmaf(e, dl, q.t);
                 if (KIND == kSearch) { q.a = fmaf(y, dl, q.a); q.b += y; }
-                if (KIND == kClippedRef) { q.a = fmaf(e, dl - fmaxf(y - C, kLow), q.a); q.b += ex2((y - C) * kLog2e); }
+                if (KIND == kClippedRef) { q.a = fmaf(e, dl - fmaxf(y - q.c, kLow), q.a); q.b += ex2((y - q.c) * kLog2e); }
             }
-    q.s = warp_sum(q.s); q.t = warp_sum(q.t); q.a = warp_sum(q.a); q.b = warp_sum(q.b);
-    if (lane == 0) { part[1][warp][0] = q.s; part[1][warp][1] = q.t; part[1][warp][2] = q.a; part[1][warp][3] = q.b; }
-    __syncthreads();
-    const float* from = part[1][lane % 16];      // each entry by two lanes
-    q.s = 0.5f * warp_sum(from[0]); q.t = 0.5f * warp_sum(from[1]); q.a = 0.5f * warp_sum(from[2]); q.b = 0.5f * warp_sum(from[3]);
+    q.s = join(q.s, false); q.t = join(q.t, false);
+    if (KIND != kClipped) { q.a = join(q.a, false); q.b = join(q.b, false); }
+    if (q.za != -kInf) q.za = max_nan(q.za, q.m + kLow);
     RowGrad g;
-    RowOut out{0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-    live = live && row_result<KIND>(r, q, w, KIND == kSearch ? 0.f : r.old_logp[row], KIND == kSearch ? 0.f : r.advantage[row], &g, &out);
-    if (threadIdx.x == 0) {
-        if (r.loss) r.loss[row] = out.loss;
-        if (r.stats) r.stats[row] = out.stats;
-    }
-    for (int j = threadIdx.x; j < r.A; j += 512) {
+    RowOut out;
+    live = row_result<KIND>(r, q, w, KIND == kSearch ? 0.f : r.old_logp[row], KIND == kSearch ? 0.f : r.advantage[row], &g, &out) && live;
+    if (tid == 0) put_out(r, row, live, out);
+    for (int j = tid; j < r.A; j += threads) {
         float o = 0.f;
         if (live && legal(bits, j)) {
             const float d = to_f32(z[j]) - g.M, dl = fmaxf(d, kLow), y = second(j);
@@ -698,39 +308,655 @@ policy_long_rows_kernel(const __grid_constant__ PolicyRows r) {
     }
 }
 
-// ---- host ---------------------------------------------------------------------------
-constexpr int kMostShared = 200 * 1024;          // of a CTA; 227 KB less the kernel's own
+// Rows without an ordinary logit - no legal action, or all of them at a type's lowest value or -inf - by one warp.
+template <typename T, int KIND>
+__device__ __noinline__ void careful_row(const PolicyRows& r, long long row) {
+    plain_row<T, KIND>(r, row, threadIdx.x % 32, 32, [](float v, bool is_max) { return is_max ? warp_max_nan(v) : team_sum(v); });
+}
 
-template <typename T, int KIND, bool WARP, bool ALIKE>
-int launch_kernel(const PolicyRows& r, RowShape sh, int threads, int ctas, cudaStream_t st) {
-    auto kernel = policy_rows_kernel<T, KIND, WARP, ALIKE>;
-    static std::atomic<int> known{0};            // registers of a thread | SMs << 16, once looked up; every device is of the same kind
-    int k = known.load(std::memory_order_acquire);
-    if (!k) {
-        int dev = 0, sms = 0;
-        cudaFuncAttributes a;
-        OB200_CUDA_OK(cudaGetDevice(&dev));
-        OB200_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-        OB200_CUDA_OK(cudaFuncGetAttributes(&a, kernel));
-        OB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
-        k = a.numRegs | sms << 16;
-        known.store(k, std::memory_order_release);
+template <typename T, int KIND>
+__global__ void __launch_bounds__(512)
+policy_long_rows_kernel(const __grid_constant__ PolicyRows r) {
+    __shared__ float part[2][16];
+    int turn = 0;
+    plain_row<T, KIND>(r, blockIdx.x, threadIdx.x, 512, [&](float v, bool is_max) {
+        v = is_max ? warp_max_nan(v) : team_sum(v);
+        if (threadIdx.x % 32 == 0) part[turn][threadIdx.x / 32] = v;
+        __syncthreads();
+        v = part[turn][threadIdx.x % 16];
+        turn ^= 1;
+        return is_max ? warp_max_nan(v) : team_sum<16>(v);
+    });
+}
+
+// ---- rows in shared memory ------------------------------------------------------------
+// How rows lie there.  A slot holds a CTA's or warp team's part of a row: a header, vectors of 16 bytes of logits, what
+// belongs to them of the second matrix, and the words of the mask.
+struct RowShape {
+    int seg;                            // vectors a CTA holds of a row
+    int x_at, mask_at, slot_bytes;      // offsets in a slot, its size
+    int slots;                          // slots in turn
+    int* error;
+};
+constexpr int kHeader = 32;             // weight, old log-probability, advantage, action; head, vectors, -, flags
+
+__device__ __forceinline__ void copy_word_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+
+// Where a row lies within its vectors: the first element's place, vectors; whether the outer vectors reach beyond the
+// matrices (else their ends hold what stands beside the row, which the first pass replaces).
+struct Place { int head, vecs; bool first_out, last_out; };
+template <typename T, int KIND, bool ALIKE>
+__device__ __forceinline__ Place place_of(const PolicyRows& r, long long row) {
+    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T);
+    Place p{0, (r.A + V - 1) / V, false, false};
+    if (ALIKE) {
+        p.head = (r.phase + (int)(row & (V - 1)) * (int)(r.z_pitch & (V - 1))) & (V - 1);
+        p.vecs = (p.head + r.A + V - 1) / V;
+        // only the rows at the ends of a matrix can reach beyond it, and with rows shorter than a vector their neighbours
+        if (row < V || row >= r.n - V) {
+            const long long lo = row * r.z_pitch - p.head, xlo = row * r.x_pitch - p.head, end = (long long)p.vecs * V;
+            p.first_out = lo < 0 || (KIND != kClipped && xlo < 0);
+            p.last_out = lo + end > (r.n - 1) * r.z_pitch + r.A || (KIND != kClipped && xlo + end > (r.n - 1) * r.x_pitch + r.A);
+        }
     }
-    const int smem = WARP ? sh.team_bytes * threads / 32 : sh.team_bytes;
-    const int by_regs = 65536 / (((k & 0xFFFF) + 7) / 8 * 8 * threads), by_smem = 224 * 1024 / (smem + 10 * 1024), by_threads = 2048 / threads;
-    int per_sm = by_regs < by_smem ? by_regs : by_smem;
-    per_sm = per_sm < by_threads ? per_sm : by_threads;
-    if (per_sm < 1) per_sm = 1;
-    const long long room = (long long)(k >> 16) * per_sm / ctas, teams = WARP ? (r.n + threads / 32 - 1) / (threads / 32) : r.n;
+    return p;
+}
+
+// A team's part of a row in its slot.
+struct Part {
+    uint8_t *zs, *xs;
+    const uint32_t* ms;                 // words of the mask from mask_first on
+    int mask_first, head, vecs, v0, v1; // this part's vectors are [v0, v1)
+    bool first_out, last_out;
+};
+
+// First pass, over vectors v0 + tid, + stride ...: the largest words; what does not count becomes the lowest value (a target
+// 0), visit counts become fp32.
+template <typename T, int KIND, bool ALIKE>
+__device__ __forceinline__ void pass_max(const PolicyRows& r, long long row, const Part& p, int tid, int stride, uint32_t* top_z, uint32_t* top_x) {
+    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
+    constexpr uint32_t kLowWord = Lowest<T>::kWord;
+    const int edge_first = p.head ? 0 : -1, edge_last = (p.head + r.A) % V ? p.vecs - 1 : -1;
+    for (int v = p.v0 + tid; v < p.v1; v += stride) {
+        uint8_t *zp = p.zs + (v - p.v0) * 16, *xp = p.xs + (v - p.v0) * XV;
+        uint32_t z[4], x[XV / 4];
+        load16(zp, z);
+        const bool edge = v == edge_first || v == edge_last;
+        if (KIND == kClippedRef || (KIND == kSearch && (r.bits || r.visits || edge)))
+#pragma unroll
+            for (int i = 0; i < XV / 16; ++i) load16(xp + 16 * i, x + 4 * i);
+        if (r.bits || edge) {
+            const int j = v * V - p.head;                   // the first element's action; below 0 in the first vector
+            if (ALIKE && ((v == 0 && p.first_out) || (v == p.vecs - 1 && p.last_out))) {
+                // not copied: it reaches beyond the matrix
+                for (int i = 0; i < V; ++i)
+                    if (j + i >= 0 && j + i < r.A) {
+                        ((T*)zp)[i] = ((const T*)r.z)[row * r.z_pitch + j + i];
+                        if (KIND == kSearch) ((uint32_t*)xp)[i] = ((const uint32_t*)r.x)[row * r.x_pitch + j + i];
+                        if (KIND == kClippedRef) ((T*)xp)[i] = ((const T*)r.x)[row * r.x_pitch + j + i];
+                    }
+                load16(zp, z);
+                if (KIND != kClipped)
+#pragma unroll
+                    for (int i = 0; i < XV / 16; ++i) load16(xp + 16 * i, x + 4 * i);
+            }
+            uint32_t on = ~0u;
+            if (r.bits) {
+                const int i = (j >> 5) - p.mask_first, most = (r.A - 1) >> 5;
+                const uint32_t lo = j < 0 ? 0u : p.ms[i], hi = (j & 31) + V > 32 && (j >> 5) < most ? p.ms[i + 1] : 0u;
+                on = __funnelshift_r(lo, hi, j & 31);
+            }
+            if (j < 0) on &= ~0u << -j;
+            if (j + V > r.A) on &= ~(~0u << (r.A - j));
+            uint32_t m[4];
+            word_masks<T>(on, m);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                z[i] = (z[i] & m[i]) | (kLowWord & ~m[i]);
+                if (KIND == kClippedRef) x[i] = (x[i] & m[i]) | (kLowWord & ~m[i]);
+            }
+            if (KIND == kSearch)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] = (on >> i) & 1u ? x[i] : 0u;
+        }
+        if (KIND == kSearch && (r.bits || r.visits || edge)) {
+            if (r.visits)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] = __float_as_uint((float)(int)x[i]);
+#pragma unroll
+            for (int i = 0; i < XV / 16; ++i) store16(xp + 16 * i, x + 4 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            z[i] = word_max<T>(z[i], kLowWord);
+            *top_z = word_max<T>(*top_z, z[i]);
+            if (KIND == kClippedRef) {
+                x[i] = word_max<T>(x[i], kLowWord);
+                *top_x = word_max<T>(*top_x, x[i]);
+            }
+        }
+        store16(zp, z);
+        if (KIND == kClippedRef) store16(xp, x);
+    }
+}
+
+// Second pass: the sums relative to q.m and q.c.
+template <typename T, int KIND>
+__device__ __forceinline__ void pass_sums(const Part& p, int tid, int stride, Sums& q) {
+    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
+    const f32x2 M = pair(-q.m, -q.m), C = pair(-q.c, -q.c), L = pair(kLog2e, kLog2e), minus = pair(-1.f, -1.f);
+    f32x2 s = 0, t = 0, a = 0, b = 0;
+#pragma unroll 2
+    for (int v = p.v0 + tid; v < p.v1; v += stride) {
+        uint32_t z[4], x[XV / 4];
+        load16(p.zs + (v - p.v0) * 16, z);
+        if (KIND != kClipped)
+#pragma unroll
+            for (int i = 0; i < XV / 16; ++i) load16(p.xs + (v - p.v0) * XV + 16 * i, x + 4 * i);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const f32x2 d = add2(elements<T>(z, i), M), e = ex2_2(mul2(d, L));
+            s = add2(s, e);
+            t = fma2(e, d, t);
+            if (KIND == kSearch) {
+                const f32x2 y = elements<float>(x, i);
+                a = fma2(y, d, a);
+                b = add2(b, y);
+            }
+            if (KIND == kClippedRef) {
+                const f32x2 c = add2(elements<T>(x, i), C);
+                b = add2(b, ex2_2(mul2(c, L)));
+                a = fma2(e, fma2(c, minus, d), a);
+            }
+        }
+    }
+    q.s = sum2(s); q.t = sum2(t); q.a = sum2(a); q.b = sum2(b);
+}
+
+// Third pass: the gradient (0 where the row is not live), to `grad` (the row's element 0 stands at grad + head), or into
+// the slot where stores of vectors are not possible.
+template <typename T, int KIND, bool ALIKE>
+__device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, int tid, int stride, bool live, const RowGrad& g, int act_e, T* grad) {
+    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
+    const f32x2 M = pair(-g.M, -g.M), C = pair(-g.C, -g.C), L = pair(kLog2e, kLog2e), minus = pair(-1.f, -1.f);
+    const f32x2 lp = pair(g.lp, g.lp), k0 = pair(g.k0, g.k0), kz = pair(g.kz, g.kz), kd = pair(g.kd, g.kd), kt = pair(-g.kt, -g.kt);
+    const int end = p.head + r.A;
+#pragma unroll 2
+    for (int v = p.v0 + tid; v < p.v1; v += stride) {
+        uint32_t z[4] = {0, 0, 0, 0}, x[XV / 4];
+        if (live) {
+            float o[V];
+            load16(p.zs + (v - p.v0) * 16, z);
+            if (KIND != kClipped)
+#pragma unroll
+                for (int i = 0; i < XV / 16; ++i) load16(p.xs + (v - p.v0) * XV + 16 * i, x + 4 * i);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const f32x2 d = add2(elements<T>(z, i), M), pr = ex2_2(fma2(d, L, lp));
+                f32x2 y = fma2(kz, d, k0);
+                if (KIND == kClippedRef) y = fma2(kd, fma2(add2(elements<T>(x, i), C), minus, d), y);
+                y = mul2(y, pr);
+                if (KIND == kSearch) y = fma2(kt, elements<float>(x, i), y);
+                halves(y, o[2 * i], o[2 * i + 1]);
+            }
+            if (KIND != kSearch && (unsigned)act_e - (unsigned)(v * V) < (unsigned)V)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (act_e == v * V + i) o[i] += g.ka;
+            if (sizeof(T) == 4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = __float_as_uint(o[i % V]);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = pack2<T>(o[(2 * i) % V], o[(2 * i + 1) % V]);
+        }
+        const int e = v * V;
+        if (!ALIKE) {
+            store16(p.zs + (v - p.v0) * 16, z);
+        } else if (e >= p.head && e + V <= end) {
+            *(uint4*)(grad + e) = make_uint4(z[0], z[1], z[2], z[3]);
+        } else {
+            uint8_t* zp = p.zs + (v - p.v0) * 16;
+            store16(zp, z);
+            for (int i = max(p.head - e, 0); i < min(V, end - e); ++i) grad[e + i] = ((const T*)zp)[i];
+        }
+    }
+}
+
+// Without vectors: what a team holds of a row, element by element, into its slot and back.
+template <typename T, int KIND>
+__device__ __forceinline__ void copy_in(const PolicyRows& r, long long row, const Part& p, int tid, int stride) {
+    constexpr int V = 16 / sizeof(T);
+    const int j0 = p.v0 * V, j1 = min(p.v1 * V, r.A);
+    for (int j = j0 + tid; j < j1; j += stride) {
+        ((T*)p.zs)[j - j0] = ((const T*)r.z)[row * r.z_pitch + j];
+        if (KIND == kSearch) ((uint32_t*)p.xs)[j - j0] = ((const uint32_t*)r.x)[row * r.x_pitch + j];
+        if (KIND == kClippedRef) ((T*)p.xs)[j - j0] = ((const T*)r.x)[row * r.x_pitch + j];
+    }
+    if (r.bits)
+        for (int i = p.mask_first + tid; i <= (j1 - 1) >> 5; i += stride) ((uint32_t*)p.ms)[i - p.mask_first] = r.bits[row * r.mask_words + i];
+}
+template <typename T>
+__device__ __forceinline__ void copy_out(const PolicyRows& r, const Part& p, int tid, int stride, T* grad) {
+    constexpr int V = 16 / sizeof(T);
+    const int j0 = p.v0 * V, j1 = min(p.v1 * V, r.A);
+    for (int j = j0 + tid; j < j1; j += stride) grad[j] = ((const T*)p.zs)[j - j0];
+}
+
+__device__ __forceinline__ float4 scalars_of(const PolicyRows& r, int kind, long long row) {
+    float4 v = make_float4(1.f, 0.f, 0.f, 0.f);
+    if (row >= r.n) return v;
+    if (r.weight) v.x = r.weight[row];
+    if (kind != kSearch) { v.y = r.old_logp[row]; v.z = r.advantage[row]; v.w = __int_as_float(r.action[row]); }
+    return v;
+}
+
+// The copies of vectors [v0, v1) of a row into a slot, announced at and counted by bar.
+template <typename T, int KIND>
+__device__ __forceinline__ void copy_vectors(const PolicyRows& r, long long row, const Place& p, int v0, int v1, uint32_t slot, int x_at, uint32_t bar, bool wanted) {
+    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
+    int lo = v0, hi = v1;
+    if (lo == 0 && p.first_out) lo = 1;
+    if (hi == p.vecs && p.last_out) --hi;
+    const int n = hi - lo;
+    if (!wanted || n <= 0) {
+        ptx::mbar_arrive(bar);
+        return;
+    }
+    ptx::mbar_arrive_expect_tx(bar, n * (KIND == kClipped ? 16 : 16 + XV));
+    const uint8_t* z = (const uint8_t*)r.z + (row * r.z_pitch - p.head + (long long)lo * V) * (int)sizeof(T);
+    ptx::bulk_g2s(slot + kHeader + (lo - v0) * 16, z, n * 16, bar);
+    if (KIND != kClipped) {
+        const uint8_t* x = (const uint8_t*)r.x + (row * r.x_pitch - p.head + (long long)lo * V) * XB;
+        ptx::bulk_g2s(slot + x_at + (lo - v0) * XV, x, n * XV, bar);
+    }
+}
+
+// ---- short rows --------------------------------------------------------------------
+// LANES lanes a row, 32 / LANES adjacent rows a warp; each warp has slots of its own and fills them itself.
+template <typename T, int KIND, int LANES, bool ALIKE>
+__global__ void __launch_bounds__(256, 2)
+policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {
+    constexpr int R = 32 / LANES;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int abort_flag;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, tid = lane % LANES, mine_of = lane / LANES;
+    const int warp_bytes = sh.slots * (R * sh.slot_bytes + 16);
+    uint8_t* const mine = smem + warp * warp_bytes;
+    const uint32_t mine_s = ptx::smem_u32(mine), bars = mine_s + sh.slots * R * sh.slot_bytes;
+    if (ALIKE && lane == 0)
+        for (int s = 0; s < sh.slots; ++s) ptx::mbar_init(bars + 16 * s, R + (r.bits ? 32 : 0));
+    if (threadIdx.x == 0) abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+
+    const long long first = ((long long)blockIdx.x * warps + warp) * R + mine_of, step = (long long)gridDim.x * warps * R;
+    // This team's row into slot s; rows beyond the last are announced too, so that the warp's barrier completes.
+    auto fill = [&](long long row, int s, float4 scalars) {
+        const int at = (s * R + mine_of) * sh.slot_bytes;
+        const uint32_t bar = bars + 16 * s;
+        const bool is = row < r.n;
+        if (r.bits) {
+            if (is)
+                for (int i = tid; i < (r.A + 31) / 32; i += LANES) copy_word_async(mine_s + at + sh.mask_at + 4 * i, r.bits + row * r.mask_words + i);
+            arrive_after_copies(bar);
+        }
+        if (tid == 0) {
+            *(float4*)(mine + at) = scalars;
+            const Place p = place_of<T, KIND, ALIKE>(r, is ? row : 0);
+            copy_vectors<T, KIND>(r, row, p, 0, p.vecs, mine_s + at, sh.x_at, bar, is && scalars.x != 0.f);
+        }
+    };
+    float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);          // scalars of the next row to be copied
+    if (ALIKE) {
+        for (int s = 0; s < sh.slots; ++s)
+            if (first - mine_of + s * step < r.n) fill(first + s * step, s, scalars_of(r, KIND, first + s * step));
+        if (tid == 0) ahead = scalars_of(r, KIND, first + sh.slots * step);
+    }
+    int slot = 0;
+    uint32_t parity = 0;
+    for (long long row = first; row - mine_of < r.n; row += step) {        // the same turns for the whole warp
+        const bool is = row < r.n;
+        uint8_t* const at = mine + (slot * R + mine_of) * sh.slot_bytes;
+        const Place pl = place_of<T, KIND, ALIKE>(r, is ? row : 0);
+        const Part p{at + kHeader, at + sh.x_at, (const uint32_t*)(at + sh.mask_at), 0, pl.head, pl.vecs, 0, is ? pl.vecs : 0, pl.first_out, pl.last_out};
+        float4 scalars;
+        if (ALIKE) {
+            if (!ptx::mbar_wait_warp(bars + 16 * slot, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+            scalars = *(const float4*)at;
+        } else {
+            scalars = scalars_of(r, KIND, row);
+            if (is && scalars.x != 0.f) copy_in<T, KIND>(r, row, p, tid, LANES);
+            __syncwarp();
+        }
+        const float w = scalars.x;
+        const int act = KIND == kSearch ? -1 : __float_as_int(scalars.w);
+        const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;       // the action's element of the row
+        bool live = is && w != 0.f, apart = false;
+        uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
+        if (live) pass_max<T, KIND, ALIKE>(r, row, p, tid, LANES, &top_z, &top_x);
+        Sums q;
+        q.m = team_max_nan<LANES>(word_top<T>(top_z));
+        q.c = KIND == kClippedRef ? team_max_nan<LANES>(word_top<T>(top_x)) : 0.f;
+        __syncwarp();
+        q.za = -kInf;
+        if (KIND != kSearch && live && act_e >= 0 && (!r.bits || (p.ms[act >> 5] >> (act & 31)) & 1u)) q.za = to_f32(((const T*)p.zs)[act_e]);
+        if (live && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2))) apart = true;
+        for (uint32_t m = __ballot_sync(~0u, apart && tid == 0); m; m &= m - 1)
+            careful_row<T, KIND>(r, __shfl_sync(~0u, row, __ffs(m) - 1));
+        live = live && !apart;
+        q.s = q.t = q.a = q.b = 0.f;
+        if (live) pass_sums<T, KIND>(p, tid, LANES, q);
+        q.s = team_sum<LANES>(q.s);
+        q.t = team_sum<LANES>(q.t);
+        if (KIND != kClipped) { q.a = team_sum<LANES>(q.a); q.b = team_sum<LANES>(q.b); }
+        RowGrad g;
+        RowOut out;
+        live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && live;
+        if (tid == 0 && is && !apart) put_out(r, row, live, out);
+        T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
+        if (!apart) pass_grad<T, KIND, ALIKE>(r, p, tid, LANES, live, g, act_e, grad);
+        if (ALIKE) {
+            // the slot's next copy comes behind what was read and written here
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (row - mine_of + sh.slots * step < r.n) {
+                fill(row + sh.slots * step, slot, ahead);
+                if (tid == 0) ahead = scalars_of(r, KIND, row + (sh.slots + 1) * step);
+            }
+        } else {
+            __syncwarp();
+            if (!apart) copy_out<T>(r, p, tid, LANES, grad);
+            __syncwarp();
+        }
+        if (++slot == sh.slots) { slot = 0; parity ^= 1; }
+    }
+    if (ALIKE && abort_flag) {                   // a wait ran out: what is still in flight is waited for once more, within the same limit
+        int none = 0;
+        for (int s = 0; s < sh.slots; ++s) ptx::mbar_wait(bars + 16 * s, s >= slot ? parity : parity ^ 1, &none);
+    }
+}
+
+// ---- rows of a CTA or a cluster ----------------------------------------------------------
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void named_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+// Bounded wait on a barrier that the cluster's other CTAs arrive at.
+__device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (uint32_t i = 0; i < ptx::kSpinLimit; ++i) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((i & 255) == 255 && *abort_flag) return false;
+    }
+    return false;
+}
+
+// The last warp copies rows ahead, the others work on them; the first of those joins their sums, and the clusters'.
+template <typename T, int KIND, bool ALIKE>
+__global__ void __launch_bounds__(512, 2)
+policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {
+    constexpr int V = 16 / sizeof(T);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float top_of[2][16][2];
+    __shared__ float part[16][8];                // the warps' sums
+    __shared__ float joined[2][8][8];            // the cluster's CTAs' sums, by turns
+    __shared__ float found[12];                  // what comes of the row: RowGrad; live; apart
+    __shared__ __align__(8) unsigned long long full_bar[4], empty_bar[4], join_bar;
+    __shared__ int abort_flag;
+    uint32_t cta, ctas;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32 - 1, threads = 32 * warps;
+    const uint32_t smem_s = ptx::smem_u32(smem), full = ptx::smem_u32(full_bar), empty = ptx::smem_u32(empty_bar), join = ptx::smem_u32(&join_bar);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < sh.slots; ++s) {
+            ptx::mbar_init(full + 8 * s, 1 + (r.bits ? 32 : 0));
+            ptx::mbar_init(empty + 8 * s, warps);
+        }
+        ptx::mbar_init(join, ctas);
+        abort_flag = 0;
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+    // the cluster's CTAs write into each other's shared memory: all of them have to be there
+    if (ctas > 1) cluster_barrier();
+    const int v0 = (int)cta * sh.seg;
+    const long long first = blockIdx.x / ctas, step = gridDim.x / ctas;
+    int slot = 0;
+    uint32_t parity = 0;
+
+    if (warp == warps) {
+        if (ALIKE) {
+            float4 ahead = scalars_of(r, KIND, first);
+            for (long long row = first; row < r.n; row += step) {
+                const float4 scalars = ahead;
+                ahead = scalars_of(r, KIND, row + step);
+                if (row >= first + sh.slots * step && !ptx::mbar_wait_warp(empty + 8 * slot, parity ^ 1, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+                uint8_t* const at = smem + slot * sh.slot_bytes;
+                const uint32_t at_s = smem_s + slot * sh.slot_bytes, bar = full + 8 * slot;
+                const Place p = place_of<T, KIND, ALIKE>(r, row);
+                const int v1 = min(p.vecs, v0 + sh.seg);
+                if (r.bits) {
+                    const int w0 = max(v0 * V - p.head, 0) >> 5, w1 = (min(v1 * V - p.head, r.A) - 1) >> 5;
+                    for (int i = w0 + lane; i <= w1; i += 32) copy_word_async(at_s + sh.mask_at + 4 * (i - w0), r.bits + row * r.mask_words + i);
+                    arrive_after_copies(bar);
+                }
+                if (lane == 0) {
+                    *(float4*)at = scalars;
+                    *(int4*)(at + 16) = make_int4(p.head, p.vecs, 0, (p.first_out ? 1 : 0) | (p.last_out ? 2 : 0));
+                    copy_vectors<T, KIND>(r, row, p, v0, v1, at_s, sh.x_at, bar, scalars.x != 0.f);
+                }
+                __syncwarp();
+                if (++slot == sh.slots) { slot = 0; parity ^= 1; }
+            }
+            if (abort_flag) {                    // a wait ran out: what is still in flight is waited for once more, within the same limit
+                int none = 0;
+                for (int s = 0; s < sh.slots; ++s) ptx::mbar_wait(full + 8 * s, s >= slot ? parity ^ 1 : parity, &none);
+            }
+        }
+    } else {
+        int turn = 0;
+        uint32_t join_parity = 0;
+        for (long long row = first; row < r.n; row += step) {
+            uint8_t* const at = smem + slot * sh.slot_bytes;
+            float4 scalars;
+            Place pl;
+            if (ALIKE) {
+                if (!ptx::mbar_wait_warp(full + 8 * slot, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+                scalars = *(const float4*)at;
+                const int4 h = *(const int4*)(at + 16);
+                pl = Place{h.x, h.y, (h.w & 1) != 0, (h.w & 2) != 0};
+            } else {
+                scalars = scalars_of(r, KIND, row);
+                pl = place_of<T, KIND, ALIKE>(r, row);
+            }
+            const Part p{at + kHeader, at + sh.x_at, (const uint32_t*)(at + sh.mask_at), max(v0 * V - pl.head, 0) >> 5, pl.head, pl.vecs,
+                         v0, min(pl.vecs, v0 + sh.seg), pl.first_out, pl.last_out};
+            const float w = scalars.x;
+            if (!ALIKE) {
+                if (w != 0.f) copy_in<T, KIND>(r, row, p, threadIdx.x, threads);
+                named_sync(1, threads);
+            }
+            const int act = KIND == kSearch ? -1 : __float_as_int(scalars.w);
+            const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;   // the action's element of the row
+            bool live = w != 0.f, apart = false;
+            RowGrad g;
+            if (live) {                          // the same in the whole team
+                uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
+                pass_max<T, KIND, ALIKE>(r, row, p, threadIdx.x, threads, &top_z, &top_x);
+                Sums q;
+                q.m = warp_max_nan(word_top<T>(top_z));
+                q.c = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
+                if (lane == 0) { top_of[turn][warp][0] = q.m; top_of[turn][warp][1] = q.c; }
+                named_sync(1, threads);
+                const int i = lane < warps ? lane : 0;
+                q.m = warp_max_nan(top_of[turn][i][0]);
+                if (KIND == kClippedRef) q.c = warp_max_nan(top_of[turn][i][1]);
+                turn ^= 1;
+                const float top = q.m, top_ref = q.c;
+                // a part without an ordinary logit: its terms vanish next to 0
+                if (q.m < Lowest<T>::kValue / 2) q.m = 0.f;
+                if (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2) q.c = 0.f;
+                pass_sums<T, KIND>(p, threadIdx.x, threads, q);
+                q.s = team_sum(q.s);
+                q.t = team_sum(q.t);
+                if (KIND != kClipped) { q.a = team_sum(q.a); q.b = team_sum(q.b); }
+                if (lane == 0) {
+                    *(float4*)part[warp] = make_float4(q.s, q.t, q.a, q.b);
+                }
+                if (warp != 0) {
+                    named_arrive(2, threads);
+                } else {
+                    named_sync(2, threads);
+                    float4 v = lane < warps ? *(const float4*)part[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    q.s = team_sum<16>(v.x); q.t = team_sum<16>(v.y);
+                    if (KIND != kClipped) { q.a = team_sum<16>(v.z); q.b = team_sum<16>(v.w); }
+                    q.za = -kInf;
+                    if (KIND != kSearch && act_e >= 0 && act_e / V >= v0 && act_e / V < p.v1 &&
+                        (!r.bits || (p.ms[(act >> 5) - p.mask_first] >> (act & 31)) & 1u))
+                        q.za = to_f32(((const T*)p.zs)[act_e - v0 * V]);
+                    float M = top, C = top_ref;
+                    if (ctas > 1) {
+                        // its sums to every CTA of the cluster, and theirs relative to the largest maxima
+                        float (*all)[8] = joined[join_parity];
+                        if (lane < (int)ctas) {
+                            uint32_t there, bar;
+                            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(ptx::smem_u32(all[cta])), "r"(lane));
+                            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(join), "r"(lane));
+                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(top), "f"(top_ref), "f"(q.s), "f"(q.t) : "memory");
+                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + 16), "f"(q.a), "f"(q.b), "f"(q.za), "f"(0.f) : "memory");
+                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+                        }
+                        if (!__all_sync(~0u, cluster_wait(join, join_parity, &abort_flag))) { abort_flag = 1; atomicExch(sh.error, 4); }
+                        join_parity ^= 1;
+                        const float* mine = all[lane < (int)ctas ? lane : 0];
+                        const float4 lo = *(const float4*)mine, hi = *(const float4*)(mine + 4);
+                        M = warp_max_nan(lo.x);
+                        C = KIND == kClippedRef ? warp_max_nan(lo.y) : 0.f;
+                        q.za = warp_max_nan(hi.z);
+                        q.s = q.t = q.a = q.b = 0.f;
+                        if (lane < (int)ctas) {
+                            const float m = lo.x < Lowest<T>::kValue / 2 ? 0.f : lo.x, c = lo.y < Lowest<T>::kValue / 2 ? 0.f : lo.y;
+                            const float d = m - M, dc = c - C, f = lo.z == 0.f ? 0.f : ex2(d * kLog2e);
+                            q.s = lo.z * f;
+                            q.t = fmaf(d, q.s, lo.w * f);
+                            if (KIND == kSearch) { q.a = fmaf(d, hi.y, hi.x); q.b = hi.y; }
+                            if (KIND == kClippedRef) { q.a = fmaf(d - dc, q.s, hi.x * f); q.b = hi.y == 0.f ? 0.f : hi.y * ex2(dc * kLog2e); }
+                        }
+                        q.s = team_sum<8>(q.s); q.t = team_sum<8>(q.t);
+                        if (KIND != kClipped) { q.a = team_sum<8>(q.a); q.b = team_sum<8>(q.b); }
+                    }
+                    q.m = M; q.c = C;
+                    apart = M < Lowest<T>::kValue / 2 || (KIND == kClippedRef && C < Lowest<T>::kValue / 2);
+                    RowOut out;
+                    live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out);
+                    if (apart) {
+                        if (cta == 0) careful_row<T, KIND>(r, row);
+                    } else if (lane == 0 && cta == 0) {
+                        put_out(r, row, live, out);
+                    }
+                    if (lane == 0) {
+                        *(float4*)found = make_float4(g.M, g.C, g.lp, g.k0);
+                        *(float4*)(found + 4) = make_float4(g.kz, g.kd, g.ka, g.kt);
+                        found[8] = live ? 1.f : 0.f;
+                        found[9] = apart ? 1.f : 0.f;
+                    }
+                }
+                named_sync(3, threads);
+                const float4 lo = *(const float4*)found, hi = *(const float4*)(found + 4);
+                g = RowGrad{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                live = found[8] != 0.f;
+                apart = found[9] != 0.f;
+            } else if (threadIdx.x == 0 && cta == 0) {
+                put_out(r, row, false, RowOut());
+            }
+            T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
+            if (!apart) pass_grad<T, KIND, ALIKE>(r, p, threadIdx.x, threads, live, g, act_e, grad);
+            if (ALIKE) {
+                // the slot's next copy comes behind what was read and written here
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(empty + 8 * slot);
+            } else {
+                named_sync(1, threads);
+                if (!apart) copy_out<T>(r, p, threadIdx.x, threads, grad);
+                named_sync(1, threads);
+            }
+            if (++slot == sh.slots) { slot = 0; parity ^= 1; }
+        }
+    }
+    __syncwarp();
+    // and none may leave while another may still write
+    if (ctas > 1) cluster_barrier();
+}
+
+// ---- host ---------------------------------------------------------------------------
+constexpr int kMostShared = 208 * 1024;          // of a CTA; 227 KB less the kernels' own
+
+// Registers of a thread | SMs << 16, looked up once for each kernel; every device is of the same kind.
+template <typename Kernel>
+int kernel_facts(Kernel kernel, std::atomic<int>* known, int* facts) {
+    *facts = known->load(std::memory_order_acquire);
+    if (*facts) return OB200_OK;
+    int dev = 0, sms = 0;
+    cudaFuncAttributes a;
+    OB200_CUDA_OK(cudaGetDevice(&dev));
+    OB200_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    OB200_CUDA_OK(cudaFuncGetAttributes(&a, kernel));
+    OB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+    *facts = a.numRegs | sms << 16;
+    known->store(*facts, std::memory_order_release);
+    return OB200_OK;
+}
+// CTAs the device holds at once.
+int resident_ctas(int facts, int threads, int smem) {
+    const int by_regs = 65536 / (((facts & 0xFFFF) + 7) / 8 * 8 * threads), by_smem = 226 * 1024 / (smem + 4 * 1024), by_threads = 2048 / threads;
+    int n = by_regs < by_smem ? by_regs : by_smem;
+    n = n < by_threads ? n : by_threads;
+    return (facts >> 16) * (n < 1 ? 1 : n);
+}
+
+template <typename T, int KIND, int LANES, bool ALIKE>
+int launch_warp_rows(const PolicyRows& r, const RowShape& sh, cudaStream_t st) {
+    constexpr int R = 32 / LANES;
+    static std::atomic<int> known{0};
+    auto kernel = policy_warp_rows_kernel<T, KIND, LANES, ALIKE>;
+    int facts;
+    if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
+    const int warp_bytes = sh.slots * (R * sh.slot_bytes + 16), fit = 104 * 1024 / warp_bytes, warps = fit < 1 ? 1 : fit > 8 ? 8 : fit;
+    const long long teams = ((long long)r.n + R * warps - 1) / (R * warps), room = resident_ctas(facts, 32 * warps, warps * warp_bytes);
+    kernel<<<(unsigned)(teams < room ? teams : room), 32 * warps, warps * warp_bytes, st>>>(r, sh);
+    OB200_LAUNCHED("policy_warp_rows_kernel");
+    return OB200_OK;
+}
+
+template <typename T, int KIND, bool ALIKE>
+int launch_cta_rows(const PolicyRows& r, const RowShape& sh, int warps, int ctas, cudaStream_t st) {
+    static std::atomic<int> known{0};
+    auto kernel = policy_cta_rows_kernel<T, KIND, ALIKE>;
+    int facts;
+    if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
+    const int threads = 32 * (warps + 1), smem = sh.slots * sh.slot_bytes;
+    const long long room = resident_ctas(facts, threads, smem) / ctas;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((teams < room ? teams : room) * ctas));
+    cfg.gridDim = dim3((unsigned)((r.n < room ? r.n : room) * ctas));
     cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cfg.attrs = attr; cfg.numAttrs = ctas > 1 ? 1 : 0;
     cudaLaunchKernelEx(&cfg, kernel, r, sh);
-    OB200_LAUNCHED("policy_rows_kernel");
+    OB200_LAUNCHED("policy_cta_rows_kernel");
     return OB200_OK;
 }
 
@@ -741,31 +967,27 @@ int launch_shape(const PolicyRows& r, cudaStream_t st) {
     RowShape sh{};
     sh.error = device_error_word();
     if (!sh.error) return set_error(OB200_ERR_CUDA, "policy loss: the device's error word is not available");
-    auto lay = [&](int ctas) {                   // fills sh but for the slots; the bytes of a slot
+    auto lay = [&](int ctas) {                   // fills sh but for the slots
         sh.seg = (vecs + ctas - 1) / ctas;
-        sh.x_at = 16 + sh.seg * 16;
+        sh.x_at = kHeader + sh.seg * 16;
         sh.mask_at = sh.x_at + sh.seg * XV;
         sh.slot_bytes = (sh.mask_at + (r.bits ? (sh.seg * V / 32 + 2) * 4 : 0) + 15) / 16 * 16;
         return sh.slot_bytes;
     };
-    auto finish = [&](int slots) {
-        sh.slots = slots;
-        sh.team_bytes = (slots * (sh.slot_bytes + 8) + 127) / 128 * 128;
-        return sh.team_bytes;
-    };
     if (r.A <= 1024) {
         lay(1);
-        const int fit = 72 * 1024 / finish(2), warps = fit < 1 ? 1 : fit > 8 ? 8 : fit;
-        return launch_kernel<T, KIND, true, ALIKE>(r, sh, 32 * warps, 1, st);
+        sh.slots = 2;
+        if (ALIKE && sh.slot_bytes <= 2400) return launch_warp_rows<T, KIND, ALIKE ? 8 : 32, ALIKE>(r, sh, st);
+        if (ALIKE && sh.slot_bytes <= 4800) return launch_warp_rows<T, KIND, ALIKE ? 16 : 32, ALIKE>(r, sh, st);
+        return launch_warp_rows<T, KIND, 32, ALIKE>(r, sh, st);
     }
     if ((long long)vecs * (16 + XV) <= 8LL * kMostShared / 2) {
         int ctas = 1;
         while (ctas < 8 && lay(ctas) > 36 * 1024) ctas *= 2;
-        if (2 * (lay(ctas) + 8) + 128 <= kMostShared) {
-            finish(sh.slot_bytes <= 20 * 1024 ? 3 : 2);
-            int threads = (sh.seg / 8 + 31) / 32 * 32;
-            threads = threads < 64 ? 64 : threads > 512 ? 512 : threads;
-            return launch_kernel<T, KIND, false, ALIKE>(r, sh, threads, ctas, st);
+        if (2 * lay(ctas) <= kMostShared) {
+            sh.slots = 2;
+            const int warps = (sh.seg + 191) / 192;
+            return launch_cta_rows<T, KIND, ALIKE>(r, sh, warps < 2 ? 2 : warps > 15 ? 15 : warps, ctas, st);
         }
     }
     policy_long_rows_kernel<T, KIND><<<(unsigned)r.n, 512, 0, st>>>(r);
