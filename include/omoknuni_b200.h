@@ -770,7 +770,7 @@ typedef struct ob200_adamw_config {
 
 /* One AdamW step over all tensors, for each element, in fp32:
  *   g = grad * grad_scale
- *   m = beta1 * m + (1 - beta1) * g,   v = beta2 * v + (1 - beta2) * g^2
+ *   m = beta1 * m + ((1 - beta1) * g),   v = beta2 * v + ((1 - beta2) * (g * g))     (fused multiply-adds)
  *   param = param * (1 - lr * weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
  * param is rounded once to its type; updates smaller than half a step of a
  * 16-bit type are lost, so keep fp32 weights where that matters.

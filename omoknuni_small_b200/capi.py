@@ -612,78 +612,81 @@ class Search:
 
 
 # ---- training operators ---------------------------------------------------------------
+def _refuse(text, *args):
+    raise Error(ERR_INVALID, text % args if args else text)
+
+
 def _require(ok, text, *args):
     if not ok:
-        raise Error(ERR_INVALID, text % args if args else text)
+        _refuse(text, *args)
 
 
-def _train_dtype(t, what):
-    import torch
-    kinds = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
-    _require(t.dtype in kinds, "%s: float32, bfloat16 or float16 is wanted, got %s", what, t.dtype)
-    return kinds[t.dtype]
+_TRAIN_TYPES = {}
 
 
-class _On:
-    """Makes a tensor's device the current one for a launch; gives the launch its current stream."""
-
-    def __init__(self, device):
+def _train_dtype(dtype, what):
+    if not _TRAIN_TYPES:
         import torch
-        _require(device.type == "cuda", "the tensors are not on a CUDA device (there is no CPU path)")
-        self.back = torch.cuda.current_device()
-        self.device, self.torch = device, torch
-
-    def __enter__(self):
-        if self.device.index != self.back:
-            self.torch.cuda.set_device(self.device)
-        return C.c_void_p(self.torch.cuda.current_stream().cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.device.index != self.back:
-            self.torch.cuda.set_device(self.back)
+        _TRAIN_TYPES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16})
+    kind = _TRAIN_TYPES.get(dtype)
+    if kind is None:
+        _refuse("%s: float32, bfloat16 or float16 is wanted, got %s", what, dtype)
+    return kind
 
 
-def _matrix(t, what, n, A, device, dtype=None):
-    """Pitch of a matrix of n rows of A adjacent elements."""
-    _require(t.dim() == 2 and t.shape[0] == n and t.shape[1] == A, "%s: shape (%d, %d) is wanted, got %s", what, n, A, tuple(t.shape))
-    _require(t.device == device, "%s is on another device than the logits", what)
-    _require(dtype is None or t.dtype == dtype, "%s: %s is wanted, got %s", what, dtype, t.dtype)
-    _require(A == 1 or t.stride(1) == 1, "%s: the elements of a row have to be adjacent", what)
-    return t.stride(0) if n > 1 else max(t.stride(0), A)
+def _launch_on(device, fn, *args):
+    """fn(*args, stream) with the tensors' device as the current one, on its current stream."""
+    import torch
+    if device.type != "cuda":
+        _refuse("the tensors are not on a CUDA device (there is no CPU path)")
+    raw, index = torch._C._cuda_getCurrentRawStream, device.index      # what torch.cuda.current_stream() wraps, a tenth of its time
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, raw(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, raw(index))
+    if rc != 0:
+        check(rc)
+
+
+def _pitch(t, what, n, A, device, dtype):
+    """Pitch of a matrix of n rows of A adjacent elements of dtype."""
+    if t.dtype != dtype or t.device != device or t.shape != (n, A):
+        _refuse("%s: a matrix (%d, %d) of %s on the logits' device is wanted, got %s of %s on %s", what, n, A, dtype, tuple(t.shape), t.dtype, t.device)
+    step, one = t.stride()
+    if one != 1 and A != 1:
+        _refuse("%s: the elements of a row have to be adjacent", what)
+    return step if n > 1 else max(step, A)
 
 
 def _vector(t, what, n, device, dtype):
     if t is None:
         return None
-    _require(t.dtype == dtype and t.device == device and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1),
-             "%s: %d adjacent values of %s on the logits' device are wanted", what, n, dtype)
+    if t.dtype != dtype or t.device != device or t.shape != (n,) or not t.is_contiguous():
+        _refuse("%s: %d adjacent values of %s on the logits' device are wanted", what, n, dtype)
     return t.data_ptr()
 
 
-def _policy_rows(logits, legal_bits, row_weight, out):
+def _policy_rows(torch, logits, legal_bits, row_weight, out):
     """The struct of both losses, and (loss, grad, stats)."""
-    import torch
-    _require(logits.dim() == 2 and logits.shape[1] > 0, "logits: a matrix of rows is wanted, got shape %s", tuple(logits.shape))
+    if logits.dim() != 2 or not logits.shape[1]:
+        _refuse("logits: a matrix of rows is wanted, got shape %s", tuple(logits.shape))
     n, A = logits.shape
-    dtype, dev = _train_dtype(logits, "logits"), logits.device
+    f32, dtype, dev = torch.float32, logits.dtype, logits.device
+    kind = _train_dtype(dtype, "logits")
     if out is None:
-        out = (torch.empty(n, dtype=torch.float32, device=dev), torch.empty((n, A), dtype=logits.dtype, device=dev),
-               torch.empty((n, 4), dtype=torch.float32, device=dev))
+        out = (torch.empty(n, dtype=f32, device=dev), torch.empty((n, A), dtype=dtype, device=dev), torch.empty((n, 4), dtype=f32, device=dev))
     loss, grad, stats = out
-    words = 0
+    bits, words = None, 0
     if legal_bits is not None:
-        _require(legal_bits.dim() == 2 and legal_bits.shape[0] == n and legal_bits.dtype == torch.int32 and legal_bits.device == dev
-                 and legal_bits.is_contiguous(), "legal_bits: a contiguous int32 matrix [%d, words] on the logits' device is wanted", n)
-        words = legal_bits.shape[1]
-    if stats is not None:
-        _require(stats.dtype == torch.float32 and stats.device == dev and tuple(stats.shape) == (n, 4) and stats.is_contiguous(),
-                 "stats: a contiguous float32 matrix [%d, 4] on the logits' device is wanted", n)
-    pitch, grad_pitch = _matrix(logits, "logits", n, A, dev), _matrix(grad, "grad", n, A, dev, logits.dtype)
-    rows = PolicyRows(logits.data_ptr(), None if legal_bits is None else legal_bits.data_ptr(),
-                      _vector(row_weight, "row_weight", n, dev, torch.float32), grad.data_ptr(),
-                      _vector(loss, "loss", n, dev, torch.float32), None if stats is None else stats.data_ptr(),
-                      pitch, grad_pitch, n, A, words, dtype)
-    return rows, out
+        if legal_bits.dim() != 2 or legal_bits.shape[0] != n or legal_bits.dtype != torch.int32 or legal_bits.device != dev or not legal_bits.is_contiguous():
+            _refuse("legal_bits: a contiguous int32 matrix [%d, words] on the logits' device is wanted", n)
+        bits, words = legal_bits.data_ptr(), legal_bits.shape[1]
+    if stats is not None and (stats.dtype != f32 or stats.device != dev or stats.shape != (n, 4) or not stats.is_contiguous()):
+        _refuse("stats: a contiguous float32 matrix [%d, 4] on the logits' device is wanted", n)
+    return PolicyRows(logits.data_ptr(), bits, _vector(row_weight, "row_weight", n, dev, f32), grad.data_ptr(), _vector(loss, "loss", n, dev, f32),
+                      None if stats is None else stats.data_ptr(), _pitch(logits, "logits", n, A, dev, dtype), _pitch(grad, "grad", n, A, dev, dtype),
+                      n, A, words, kind), out
 
 
 def policy_loss_search(logits, target, legal_bits=None, row_weight=None, entropy_coef=0.0, out=None):
@@ -694,12 +697,11 @@ def policy_loss_search(logits, target, legal_bits=None, row_weight=None, entropy
     stats [n, 4] float32: cross entropy, entropy, sum of the target, log-sum-exp); `out`: the three to write into (loss and
     stats may be None, grad may be the logits).  With logits from autograd: torch.autograd.backward(logits, grad)."""
     import torch
-    rows, out = _policy_rows(logits, legal_bits, row_weight, out)
-    kind = {torch.int32: TARGET_VISITS, torch.float32: TARGET_PROBS}.get(target.dtype)
-    _require(kind is not None, "target: int32 or float32 is wanted, got %s", target.dtype)
-    pitch = _matrix(target, "target", rows.n, rows.n_actions, logits.device)
-    with _On(logits.device) as stream:
-        check(lib().ob200_launch_policy_loss_search(C.byref(rows), target.data_ptr(), pitch, kind, entropy_coef, stream))
+    rows, out = _policy_rows(torch, logits, legal_bits, row_weight, out)
+    visits = target.dtype == torch.int32
+    pitch = _pitch(target, "target", rows.n, rows.n_actions, logits.device, torch.int32 if visits else torch.float32)
+    _launch_on(logits.device, lib().ob200_launch_policy_loss_search, rows, target.data_ptr(), pitch,
+               TARGET_VISITS if visits else TARGET_PROBS, entropy_coef)
     return out
 
 
@@ -709,17 +711,13 @@ def policy_loss_clipped(logits, action, old_logp, advantage, legal_bits=None, re
     (ob200_launch_policy_loss_clipped).  action [n] int32, old_logp and advantage [n] float32, ref_logits [n, A] of the
     logits' type or None; the rest as policy_loss_search.  stats: log-probability of the action, ratio, KL, entropy."""
     import torch
-    rows, out = _policy_rows(logits, legal_bits, row_weight, out)
-    dev, n = logits.device, rows.n
-    ref, ref_pitch = None, 0
+    rows, out = _policy_rows(torch, logits, legal_bits, row_weight, out)
+    dev, n, ref, ref_pitch = logits.device, rows.n, None, 0
     if ref_logits is not None:
-        ref, ref_pitch = ref_logits.data_ptr(), _matrix(ref_logits, "ref_logits", n, rows.n_actions, dev, logits.dtype)
-    _require(action is not None and old_logp is not None and advantage is not None, "action, old_logp and advantage are wanted")
+        ref, ref_pitch = ref_logits.data_ptr(), _pitch(ref_logits, "ref_logits", n, rows.n_actions, dev, logits.dtype)
     act, old, adv = (_vector(action, "action", n, dev, torch.int32), _vector(old_logp, "old_logp", n, dev, torch.float32),
                      _vector(advantage, "advantage", n, dev, torch.float32))
-    with _On(dev) as stream:
-        check(lib().ob200_launch_policy_loss_clipped(C.byref(rows), act, old, adv, ref, ref_pitch, clip_low, clip_high, kl_coef,
-                                                     entropy_coef, stream))
+    _launch_on(dev, lib().ob200_launch_policy_loss_clipped, rows, act, old, adv, ref, ref_pitch, clip_low, clip_high, kl_coef, entropy_coef)
     return out
 
 
@@ -729,7 +727,7 @@ def _same_kind(tensors, what):
     for i, t in enumerate(tensors):
         _require(t.dtype == first.dtype and t.device == first.device, "%s %d: type or device differs from the first one's", what, i)
         _require(t.is_contiguous(), "%s %d is not contiguous", what, i)
-    return _train_dtype(first, what), first.device
+    return _train_dtype(first.dtype, what), first.device
 
 
 class GradNorm:
@@ -753,9 +751,8 @@ class GradNorm:
             e.grad, e.numel = g.data_ptr(), g.numel()
 
     def run(self, max_norm=float("inf")):
-        with _On(self.device) as stream:
-            check(lib().ob200_launch_grad_norm(self.table, len(self.table), self.dtype, max_norm, self.workspace.data_ptr(),
-                                               self.out.data_ptr(), stream))
+        _launch_on(self.device, lib().ob200_launch_grad_norm, self.table, len(self.table), self.dtype, max_norm, self.workspace.data_ptr(),
+                   self.out.data_ptr())
         return self.out
 
 
@@ -809,7 +806,8 @@ class AdamW:
         self.steps = 0
 
     def _scalar(self, t, what, dtype):
-        _require(t.dtype == dtype and t.device == self.device and t.numel() == 1, "AdamW: %s is one %s on the weights' device", what, dtype)
+        if t.dtype != dtype or t.device != self.device or t.numel() != 1:
+            _refuse("AdamW: %s is one %s on the weights' device", what, dtype)
         return t.data_ptr()
 
     def step(self, lr, step=None, grad_scale=None):
@@ -819,15 +817,14 @@ class AdamW:
         import torch
         c = self.cfg
         c.grad_scale = None if grad_scale is None else self._scalar(grad_scale, "grad_scale", torch.float32)
-        if torch.is_tensor(lr):
+        if isinstance(lr, torch.Tensor):
             c.lr, c.lr_device = 0.0, self._scalar(lr, "lr", torch.float32)
         else:
             c.lr, c.lr_device = lr, None
-        if torch.is_tensor(step):
+        if isinstance(step, torch.Tensor):
             c.step, c.step_device = 0, self._scalar(step, "step", torch.int32)
         else:
             c.step, c.step_device = self.steps + 1 if step is None else step, None
-        with _On(self.device) as stream:
-            check(lib().ob200_launch_adamw(self.table, len(self.table), C.byref(c), stream))
-        if not torch.is_tensor(step):
+        _launch_on(self.device, lib().ob200_launch_adamw, self.table, len(self.table), c)
+        if c.step:
             self.steps = c.step

@@ -1,34 +1,39 @@
 // The weight update: the 2-norm of all gradients of a network with the factor that clips it, and one AdamW step over all
 // its tensors, states in fp32 or in e4m3 with a scale per 256 elements.
 //
-// Both go over the tensors in chunks of 2,048 elements, a CTA each; the list of tensors travels as a kernel parameter
-// (up to 32 KB), so that a call needs no device table, no copy and no memory of its own and can be captured.
+// Both go over the tensors in chunks, a CTA each at a time; the list of tensors travels as a kernel parameter (up to
+// 32 KB), so that a call needs no device table, no copy and no memory of its own and can be captured.  Both are bound by
+// memory: every gradient, weight and state is read once and written once.
 #include "common.h"
+#include "packed_f32.cuh"
 #include <algorithm>
 #include <cmath>
 #include <memory>
 #include <new>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 namespace ob200 {
 namespace {
 
 constexpr int kBlock = 256;              // elements that share the scales of 8-bit states
-constexpr int kChunk = 2048;             // elements of a CTA: eight warps, a block each
+// Elements of a CTA of AdamW: eight warps, a block each, or two where the states are codes (what a CTA costs besides its
+// elements is a fifth of the instructions with one).
+template <int BITS> constexpr int kChunk = BITS == 8 ? 4096 : 2048;
+template <typename G> constexpr int kNormChunk = 1024 * (16 / (int)sizeof(G));    // of a CTA's turn of the norm: 64 bytes a thread
 constexpr float kE4m3Max = 448.f, kE4m3Least = 0x1p-9f, kScaleFloor = 0x1p-110f;
-constexpr int kNormCtas = 592;           // partial sums of the norm: four CTAs per SM
+constexpr int kNormCtas = 1184;          // partial sums of the norm: eight CTAs per SM
 
 struct Entry {
     void* p; const void* g; void* m; void* v;
     float *ms, *vs;
     long long n;
-    int chunk0;                          // first chunk of this tensor within the launch
     float decay;
+    int vec;                             // whether four adjacent elements may be moved at once
 };
-template <int N> struct Table { int count, chunks; Entry e[N]; };
-constexpr int kSmallTable = 48, kLargeTable = 500;
+// chunk0[i]: the first chunk of tensor i within the launch, rising (tensors without elements are not listed).
+template <int N> struct Table { int count, chunks; int chunk0[N]; Entry e[N]; };
+constexpr int kSmallTable = 48, kMiddleTable = 160, kLargeTable = 450;
 static_assert(sizeof(Table<kLargeTable>) + 128 <= 32764, "the table has to fit the kernel parameters");
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -39,57 +44,118 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// The tensor that holds a chunk: the last one whose first chunk is not behind it (tensors without elements are not listed).
+// The tensor that holds a chunk.  (Lanes that count the places behind theirs read parameter memory one after the other:
+// AdamW over 130 tensors took 125 us that way, 92 us with steps that all lanes take together.)
 template <int N>
-__device__ __forceinline__ const Entry& entry_of(const Table<N>& t, int chunk) {
+__device__ __forceinline__ int entry_of(const Table<N>& t, int chunk) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (t.e[mid].chunk0 <= chunk) lo = mid; else hi = mid - 1;
+        if (t.chunk0[mid] <= chunk) lo = mid; else hi = mid - 1;
     }
-    return t.e[lo];
+    return lo;
+}
+
+// Four adjacent elements as fp32, and back.
+__device__ __forceinline__ void load4(const float* p, float* v) {
+    const float4 q = *(const float4*)p;
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, float* v) {
+    const uint2 q = *(const uint2*)p;
+    v[0] = __uint_as_float(q.x << 16); v[1] = __uint_as_float(q.x & 0xFFFF0000u);
+    v[2] = __uint_as_float(q.y << 16); v[3] = __uint_as_float(q.y & 0xFFFF0000u);
+}
+__device__ __forceinline__ void load4(const __half* p, float* v) {
+    const uint2 q = *(const uint2*)p;
+    const float2 a = __half22float2(*(const __half2*)&q.x), b = __half22float2(*(const __half2*)&q.y);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+// 16 bytes of T as fp32.
+__device__ __forceinline__ void load16(const float* p, float* v) { load4(p, v); }
+__device__ __forceinline__ void load16(const __nv_bfloat16* p, float* v) {
+    const uint4 q = *(const uint4*)p;
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+}
+__device__ __forceinline__ void load16(const __half* p, float* v) {
+    const uint4 q = *(const uint4*)p;
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*(const __half2*)&w[i]);
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void store4(float* p, const float* v) { *(float4*)p = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *(uint2*)p = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+}
+__device__ __forceinline__ void store4(__half* p, const float* v) {
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    *(uint2*)p = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
 }
 
 // ---- norm ----------------------------------------------------------------------
-// Squares and a thread's sums in fp32 (a thread sees a few hundred elements), everything beyond a thread in fp64.
+// Sum of a thread's value over the CTA of eight warps, in thread 0.
+__device__ __forceinline__ double cta_sum(double v) {
+    __shared__ double warp_sum[8];
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = v;
+    __syncthreads();
+    double a = 0.0;
+    if (threadIdx.x == 0)
+        for (int w = 0; w < 8; ++w) a += warp_sum[w];
+    return a;
+}
+
+// Squares and a thread's sums over a chunk (16 or 32 elements) in fp32, everything beyond in fp64.
 template <typename G, int N>
 __global__ void __launch_bounds__(256)
 grad_norm_part_kernel(const __grid_constant__ Table<N> t, double* __restrict__ part) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // grad_norm_finish_kernel waits for the whole grid
+    constexpr int V = 16 / sizeof(G);
     double sum = 0.0;
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const Entry& e = entry_of(t, c);
-        const long long at = (long long)(c - e.chunk0) * kChunk;
-        const G* g = (const G*)e.g;
-        float s = 0.f;
-        for (int i = threadIdx.x; i < kChunk && at + i < e.n; i += 256) {
-            const float v = to_f32(g[at + i]);
-            s = fmaf(v, v, s);
+    int c = (int)((long long)t.chunks * blockIdx.x / gridDim.x);
+    const int end = (int)((long long)t.chunks * (blockIdx.x + 1) / gridDim.x);
+    for (int i = entry_of(t, c); c < end; ++c) {
+        while (i + 1 < t.count && t.chunk0[i + 1] <= c) ++i;
+        const Entry& e = t.e[i];
+        const long long at = (long long)(c - t.chunk0[i]) * kNormChunk<G>;
+        const G* g = (const G*)e.g + at;
+        const int left = (int)min((long long)kNormChunk<G>, e.n - at);
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (e.vec && left == kNormChunk<G>) {
+            float v[4][V];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load16(g + V * (threadIdx.x + 256 * i), v[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < V; ++k) s[k % 4] = fmaf(v[i][k], v[i][k], s[k % 4]);
+        } else {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < left; i += 256) {
+                const float v = to_f32(g[i]);
+                s[0] = fmaf(v, v, s[0]);
+            }
         }
-        sum += (double)s;
+        sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
     }
-    __shared__ double warp_sum[8];
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double a = 0.0;
-        for (int w = 0; w < 8; ++w) a += warp_sum[w];
-        part[blockIdx.x] = a;
-    }
+    sum = cta_sum(sum);
+    if (threadIdx.x == 0) part[blockIdx.x] = sum;
 }
 
 __global__ void __launch_bounds__(256)
-grad_norm_finish_kernel(const double* __restrict__ part, int n, float max_norm, float* __restrict__ out) {
+grad_norm_finish_kernel(const double* part, int n, float max_norm, float* out) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     double sum = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) sum += part[i];
-    __shared__ double warp_sum[8];
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = sum;
-    __syncthreads();
+    sum = cta_sum(sum);
     if (threadIdx.x) return;
-    double a = 0.0;
-    for (int w = 0; w < 8; ++w) a += warp_sum[w];
-    const double norm = sqrt(a);
+    const double norm = sqrt(sum);
     out[0] = (float)norm;
     // an infinite norm gives NaN, not 0: the step is to be left out, not made with zeroed gradients
     out[1] = !isfinite((float)norm) ? __int_as_float(0x7fc00000) : norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f;
@@ -104,21 +170,49 @@ struct Step {
     const float* grad_scale; const float* lr_device; const int32_t* step_device;
 };
 
-__device__ __forceinline__ float decode_e4m3(uint8_t c) {
-    __nv_fp8_e4m3 v;
-    v.__x = c;
-    return (float)v;
+// Two codes to two fp32 (exact), and two fp32 to two codes.
+__device__ __forceinline__ void decode2(uint32_t codes, float& a, float& b) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)codes));
+    const float2 f = __half22float2(*(const __half2*)&h);
+    a = f.x; b = f.y;
 }
-__device__ __forceinline__ uint8_t encode_e4m3(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint32_t encode2(float a, float b) {
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(b), "f"(a));
+    return c;
+}
 
 // Largest of the warp's non-negative values (NaN is larger than all).
 __device__ __forceinline__ float warp_max(float v) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(v))); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float larger(float a, float b) { return max_nan(a, fabsf(b)); }
 
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A warp per block of 256, NB blocks a warp: a lane has elements 4 lane + {0..3} and 128 + 4 lane + {0..3}, or, where a
+// tensor's start does not allow four at once and in its last block, lane + 32 i.
+// The moments are fused multiply-adds, beta m + ((1 - beta) g) and beta v + ((1 - beta) (g g)), every other product rounded, so
+// that the codes of 8-bit states are a function of the inputs alone.
 template <typename P, typename G, int BITS, int N>
 __global__ void __launch_bounds__(256)
 adamw_kernel(const __grid_constant__ Table<N> t, const __grid_constant__ Step k) {
+    constexpr int NB = kChunk<BITS> / (8 * kBlock);
+    const int at_entry = entry_of(t, blockIdx.x);
+    const Entry& e = t.e[at_entry];
+    const int lane = threadIdx.x % 32;
+    const long long first = ((long long)((int)blockIdx.x - t.chunk0[at_entry]) * 8 + threadIdx.x / 32) * NB;
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // until here nothing but the parameters was read
     const float gs = k.grad_scale ? *k.grad_scale : 1.f;
-    if (!isfinite(gs)) return;
+    if (!isfinite(gs) || first * kBlock >= e.n) return;
     const float lr = k.lr_device ? *k.lr_device : k.lr;
     float rate = k.rate, root = k.root;
     if (k.step_device) {
@@ -127,54 +221,138 @@ adamw_kernel(const __grid_constant__ Table<N> t, const __grid_constant__ Step k)
         root = (float)(1.0 / sqrt(1.0 - pow(k.beta2_d, step)));
     }
     rate *= lr;
-    const Entry& e = entry_of(t, blockIdx.x);
-    const int lane = threadIdx.x % 32;
-    const long long block = (long long)((int)blockIdx.x - e.chunk0) * (kChunk / kBlock) + threadIdx.x / 32;
-    const long long at = block * kBlock;
-    if (at >= e.n) return;
-    const int left = (int)min((long long)kBlock, e.n - at);
-    const float keep = fmaf(-lr, e.decay, 1.f);
-    P* p = (P*)e.p + at;
-    const G* g = (const G*)e.g + at;
-    float ms = 0.f, vs = 0.f;
-    if (BITS == 8) { ms = e.ms[block]; vs = e.vs[block]; }
-    float mm[8], rr[8], m_top = 0.f, r_top = 0.f;
+    float pe[NB][8], ge[NB][8], m[NB][8], v[NB][8], ms[NB], vs[NB];
+    uint32_t mc[NB][2], vc[NB][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int j = lane + 32 * i;
-        mm[i] = rr[i] = 0.f;
-        if (j >= left) continue;
-        float m, v;
-        if (BITS == 32) { m = ((const float*)e.m)[at + j]; v = ((const float*)e.v)[at + j]; }
-        else {
-            m = __fmul_rn(decode_e4m3(((const uint8_t*)e.m)[at + j]), ms);
-            const float r = __fmul_rn(decode_e4m3(((const uint8_t*)e.v)[at + j]), vs);
-            v = __fmul_rn(r, r);
+    for (int b = 0; b < NB; ++b) {
+        const long long at = (first + b) * kBlock;
+        const int left = (int)max(0LL, min((long long)kBlock, e.n - at));
+        const P* p = (const P*)e.p + at;
+        const G* g = (const G*)e.g + at;
+        const float *m32 = (const float*)e.m + at, *v32 = (const float*)e.v + at;
+        const uint8_t *m8 = (const uint8_t*)e.m + at, *v8 = (const uint8_t*)e.v + at;
+        if (e.vec && left == kBlock) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int j = 128 * h + 4 * lane;
+                load4(p + j, pe[b] + 4 * h);
+                load4(g + j, ge[b] + 4 * h);
+                if (BITS == 32) { load4(m32 + j, m[b] + 4 * h); load4(v32 + j, v[b] + 4 * h); }
+                else { mc[b][h] = *(const uint32_t*)(m8 + j); vc[b][h] = *(const uint32_t*)(v8 + j); }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mc[b][h] = vc[b][h] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = lane + 32 * i;
+                const bool is = j < left;
+                pe[b][i] = is ? to_f32(p[j]) : 0.f;
+                ge[b][i] = is ? to_f32(g[j]) : 0.f;
+                if (BITS == 32) { m[b][i] = is ? m32[j] : 0.f; v[b][i] = is ? v32[j] : 0.f; }
+                else if (is) { mc[b][i / 4] |= (uint32_t)m8[j] << (8 * (i % 4)); vc[b][i / 4] |= (uint32_t)v8[j] << (8 * (i % 4)); }
+            }
         }
-        const float gr = __fmul_rn(to_f32(g[j]), gs);
-        m = __fadd_rn(__fmul_rn(m, k.beta1), __fmul_rn(gr, k.one_beta1));
-        v = __fadd_rn(__fmul_rn(v, k.beta2), __fmul_rn(__fmul_rn(gr, gr), k.one_beta2));
-        const float r = __fsqrt_rn(v);
-        p[j] = from_f32<P>(fmaf(-rate, __fdividef(m, fmaf(r, root, k.eps)), to_f32(p[j]) * keep));
-        if (BITS == 32) { ((float*)e.m)[at + j] = m; ((float*)e.v)[at + j] = v; }
-        mm[i] = m; rr[i] = r;
-        m_top = __uint_as_float(max(__float_as_uint(m_top), __float_as_uint(fabsf(m))));
-        r_top = __uint_as_float(max(__float_as_uint(r_top), __float_as_uint(fabsf(r))));
+        if (BITS == 8 && left > 0) { ms[b] = e.ms[first + b]; vs[b] = e.vs[first + b]; }
     }
-    if (BITS == 8) {
+    const f32x2 gs2 = pair(gs, gs), b1 = pair(k.beta1, k.beta1), ob1 = pair(k.one_beta1, k.one_beta1), b2 = pair(k.beta2, k.beta2),
+                ob2 = pair(k.one_beta2, k.one_beta2), root2 = pair(root, root), eps2 = pair(k.eps, k.eps), rate2 = pair(-rate, -rate);
+    const float keep = fmaf(-lr, e.decay, 1.f);
+    const f32x2 keep2 = pair(keep, keep);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const long long at = (first + b) * kBlock;
+        const int left = (int)max(0LL, min((long long)kBlock, e.n - at));
+        if (left == 0) break;
+        float r[8], m_top = 0.f, r_top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            f32x2 m2, v2;
+            if (BITS == 32) {
+                m2 = pair(m[b][i], m[b][i + 1]);
+                v2 = pair(v[b][i], v[b][i + 1]);
+            } else {
+                float x, y;
+                decode2(mc[b][i / 4] >> (8 * (i % 4)), x, y);
+                m2 = mul2(pair(x, y), pair(ms[b], ms[b]));
+                decode2(vc[b][i / 4] >> (8 * (i % 4)), x, y);
+                v2 = mul2(pair(x, y), pair(vs[b], vs[b]));
+                v2 = mul2(v2, v2);
+            }
+            const f32x2 g2 = mul2(pair(ge[b][i], ge[b][i + 1]), gs2);
+            m2 = fma2(b1, m2, mul2(g2, ob1));
+            v2 = fma2(b2, v2, mul2(mul2(g2, g2), ob2));
+            float x, y;
+            halves(v2, v[b][i], v[b][i + 1]);
+            halves(m2, m[b][i], m[b][i + 1]);
+            r[i] = __fsqrt_rn(v[b][i]);
+            r[i + 1] = __fsqrt_rn(v[b][i + 1]);
+            halves(fma2(pair(r[i], r[i + 1]), root2, eps2), x, y);
+            halves(fma2(rate2, mul2(m2, pair(rcp(x), rcp(y))), mul2(pair(pe[b][i], pe[b][i + 1]), keep2)), pe[b][i], pe[b][i + 1]);
+            if (BITS == 8) {
+                m_top = larger(larger(m_top, m[b][i]), m[b][i + 1]);
+                r_top = larger(larger(r_top, r[i]), r[i + 1]);
+            }
+        }
+        P* p = (P*)e.p + at;
+        float *m32 = (float*)e.m + at, *v32 = (float*)e.v + at;
+        uint8_t *m8 = (uint8_t*)e.m + at, *v8 = (uint8_t*)e.v + at;
+        const bool vec = e.vec && left == kBlock;
+        if (vec) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int j = 128 * h + 4 * lane;
+                store4(p + j, pe[b] + 4 * h);
+                if (BITS == 32) { store4(m32 + j, m[b] + 4 * h); store4(v32 + j, v[b] + 4 * h); }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = lane + 32 * i;
+                if (j >= left) continue;
+                p[j] = from_f32<P>(pe[b][i]);
+                if (BITS == 32) { m32[j] = m[b][i]; v32[j] = v[b][i]; }
+            }
+        }
+        if (BITS == 32) continue;
         m_top = warp_max(m_top); r_top = warp_max(r_top);
         if (m_top < kScaleFloor) m_top = kScaleFloor;
         if (r_top < kScaleFloor) r_top = kScaleFloor;
         const float mi = __fdiv_rn(kE4m3Max, m_top), ri = __fdiv_rn(kE4m3Max, r_top);
+        const f32x2 mi2 = pair(mi, mi), ri2 = pair(ri, ri);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int j = lane + 32 * i;
-            if (j >= left) continue;
-            ((uint8_t*)e.m)[at + j] = encode_e4m3(__fmul_rn(mm[i], mi));
-            const float x = __fmul_rn(rr[i], ri);
-            ((uint8_t*)e.v)[at + j] = encode_e4m3(rr[i] > 0.f && x < kE4m3Least ? kE4m3Least : x);
+        for (int h = 0; h < 2; ++h) {
+            uint32_t c[4];
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                float x, y;
+                halves(mul2(pair(m[b][4 * h + i], m[b][4 * h + i + 1]), mi2), x, y);
+                c[i] = encode2(x, y);
+                halves(mul2(pair(r[4 * h + i], r[4 * h + i + 1]), ri2), x, y);
+                if (r[4 * h + i] > 0.f) x = max_nan(x, kE4m3Least);
+                if (r[4 * h + i + 1] > 0.f) y = max_nan(y, kE4m3Least);
+                c[i + 1] = encode2(x, y);
+            }
+            mc[b][h] = __byte_perm(c[0], c[2], 0x5410);
+            vc[b][h] = __byte_perm(c[1], c[3], 0x5410);
         }
-        if (lane == 0) { e.ms[block] = __fdiv_rn(m_top, kE4m3Max); e.vs[block] = __fdiv_rn(r_top, kE4m3Max); }
+        if (vec) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int j = 128 * h + 4 * lane;
+                *(uint32_t*)(m8 + j) = mc[b][h];
+                *(uint32_t*)(v8 + j) = vc[b][h];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = lane + 32 * i;
+                if (j >= left) continue;
+                m8[j] = (uint8_t)(mc[b][i / 4] >> (8 * (i % 4)));
+                v8[j] = (uint8_t)(vc[b][i / 4] >> (8 * (i % 4)));
+            }
+        }
+        if (lane == 0) { e.ms[first + b] = __fdiv_rn(m_top, kE4m3Max); e.vs[first + b] = __fdiv_rn(r_top, kE4m3Max); }
     }
 }
 
@@ -183,29 +361,33 @@ int elem_bytes(int dtype) { return dtype == OB200_DTYPE_F32 ? 4 : 2; }
 bool is_dtype(int d) { return d == OB200_DTYPE_BF16 || d == OB200_DTYPE_F16 || d == OB200_DTYPE_F32; }
 
 // Fills t with tensors [*next, n) as far as they fit; false when there was nothing left to take.
+// chunk: elements; wide: bytes that p, g and the states have to be aligned to for four elements at once, 1 where it does not matter.
+struct Wide { uintptr_t p, g, state; };
 template <int N>
-bool fill_table(Table<N>* t, const ob200_train_tensor* in, int n, int* next, long long* chunks) {
+bool fill_table(Table<N>* t, const ob200_train_tensor* in, int n, int chunk, Wide wide, int* next, long long* chunks) {
     t->count = 0;
     *chunks = 0;
     for (; *next < n && t->count < N; ++*next) {
         const ob200_train_tensor& a = in[*next];
         if (a.numel == 0) continue;
-        const long long c = (a.numel + kChunk - 1) / kChunk;
+        const long long c = (a.numel + chunk - 1) / chunk;
         if (t->count && *chunks + c > 0x7fffffffLL) break;   // the rest in another launch
-        t->e[t->count++] = Entry{a.param, a.grad, a.exp_avg, a.exp_avg_sq, a.exp_avg_scale, a.exp_avg_sq_scale, a.numel, (int)*chunks, a.weight_decay};
+        t->chunk0[t->count] = (int)*chunks;
+        t->e[t->count++] = Entry{a.param, a.grad, a.exp_avg, a.exp_avg_sq, a.exp_avg_scale, a.exp_avg_sq_scale, a.numel, a.weight_decay,
+                               (((uintptr_t)a.param & (wide.p - 1)) | ((uintptr_t)a.grad & (wide.g - 1)) | (((uintptr_t)a.exp_avg | (uintptr_t)a.exp_avg_sq) & (wide.state - 1))) == 0};
         *chunks += c;
     }
     t->chunks = (int)*chunks;
     return t->count > 0;
 }
 
-constexpr long long kMostElements = 0x7fffffffLL * kChunk;
+constexpr long long kMostElements = 0x7fffffffLL * 2048;
 
 int check_list(const char* who, const ob200_train_tensor* t, int n) {
     if (n < 0 || (n > 0 && !t)) return set_error(OB200_ERR_INVALID, "%s: null tensors or a negative count", who);
     for (int i = 0; i < n; ++i) {
         if (t[i].numel < 0) return set_error(OB200_ERR_INVALID, "%s: tensor %d has a negative size", who, i);
-        if (t[i].numel > kMostElements) return set_error(OB200_ERR_TOO_LARGE, "%s: tensor %d has over 2^42 elements", who, i);
+        if (t[i].numel > kMostElements) return set_error(OB200_ERR_TOO_LARGE, "%s: tensor %d has too many elements", who, i);
         if (t[i].numel && !t[i].grad) return set_error(OB200_ERR_INVALID, "%s: tensor %d has no gradient", who, i);
     }
     return OB200_OK;
@@ -216,7 +398,7 @@ int norm_launches(const ob200_train_tensor* tensors, int n, double* part, int* p
     Table<N> t;
     int next = 0;
     long long chunks;
-    while (fill_table(&t, tensors, n, &next, &chunks)) {
+    while (fill_table(&t, tensors, n, kNormChunk<G>, Wide{1, 16, 1}, &next, &chunks)) {
         // each launch its own partial sums; lists of more than one launch share the places out
         const int room = kNormCtas - *parts, more = (n - next + N - 1) / N;
         if (room < 1) return set_error(OB200_ERR_TOO_LARGE, "ob200_launch_grad_norm: too many tensors");
@@ -228,13 +410,19 @@ int norm_launches(const ob200_train_tensor* tensors, int n, double* part, int* p
     return OB200_OK;
 }
 
+template <typename G>
+int norm_typed(const ob200_train_tensor* tensors, int n, double* part, int* parts, cudaStream_t st) {
+    if (n <= kSmallTable) return norm_launches<G, kSmallTable>(tensors, n, part, parts, st);
+    return n <= kMiddleTable ? norm_launches<G, kMiddleTable>(tensors, n, part, parts, st) : norm_launches<G, kLargeTable>(tensors, n, part, parts, st);
+}
+
 template <typename P, typename G, int BITS, int N>
 int adamw_launches(const ob200_train_tensor* tensors, int n, const Step& k, cudaStream_t st) {
     Table<N> t;
     int next = 0;
     long long chunks;
-    while (fill_table(&t, tensors, n, &next, &chunks)) {
-        adamw_kernel<P, G, BITS, N><<<(unsigned)chunks, 256, 0, st>>>(t, k);
+    while (fill_table(&t, tensors, n, kChunk<BITS>, Wide{4 * sizeof(P), 4 * sizeof(G), BITS == 32 ? 16 : 4}, &next, &chunks)) {
+        OB200_CUDA_OK(launch_dependent(adamw_kernel<P, G, BITS, N>, dim3((unsigned)chunks), dim3(256), 0, st, t, k));
         OB200_LAUNCHED("adamw_kernel");
     }
     return OB200_OK;
@@ -244,6 +432,8 @@ template <typename P, typename G>
 int adamw_typed(const ob200_train_tensor* tensors, int n, int bits, const Step& k, cudaStream_t st) {
     if (n <= kSmallTable)
         return bits == 8 ? adamw_launches<P, G, 8, kSmallTable>(tensors, n, k, st) : adamw_launches<P, G, 32, kSmallTable>(tensors, n, k, st);
+    if (n <= kMiddleTable)
+        return bits == 8 ? adamw_launches<P, G, 8, kMiddleTable>(tensors, n, k, st) : adamw_launches<P, G, 32, kMiddleTable>(tensors, n, k, st);
     return bits == 8 ? adamw_launches<P, G, 8, kLargeTable>(tensors, n, k, st) : adamw_launches<P, G, 32, kLargeTable>(tensors, n, k, st);
 }
 
@@ -300,15 +490,12 @@ int ob200_launch_grad_norm(const ob200_train_tensor* tensors, int32_t n_tensors,
     cudaStream_t st = as_stream(stream);
     double* part = (double*)workspace;
     int parts = 0, rc;
-    const bool small = n_tensors <= kSmallTable;
-    if (grad_dtype == OB200_DTYPE_BF16)
-        rc = small ? norm_launches<__nv_bfloat16, kSmallTable>(tensors, n_tensors, part, &parts, st) : norm_launches<__nv_bfloat16, kLargeTable>(tensors, n_tensors, part, &parts, st);
-    else if (grad_dtype == OB200_DTYPE_F16)
-        rc = small ? norm_launches<__half, kSmallTable>(tensors, n_tensors, part, &parts, st) : norm_launches<__half, kLargeTable>(tensors, n_tensors, part, &parts, st);
-    else
-        rc = small ? norm_launches<float, kSmallTable>(tensors, n_tensors, part, &parts, st) : norm_launches<float, kLargeTable>(tensors, n_tensors, part, &parts, st);
+    if (grad_dtype == OB200_DTYPE_BF16) rc = norm_typed<__nv_bfloat16>(tensors, n_tensors, part, &parts, st);
+    else if (grad_dtype == OB200_DTYPE_F16) rc = norm_typed<__half>(tensors, n_tensors, part, &parts, st);
+    else rc = norm_typed<float>(tensors, n_tensors, part, &parts, st);
     if (rc) return rc;
-    grad_norm_finish_kernel<<<1, 256, 0, st>>>(part, parts, max_norm, out);
+    if (parts) OB200_CUDA_OK(launch_dependent(grad_norm_finish_kernel, dim3(1), dim3(256), 0, st, (const double*)part, parts, max_norm, out));
+    else grad_norm_finish_kernel<<<1, 256, 0, st>>>(part, 0, max_norm, out);
     OB200_LAUNCHED("grad_norm_finish_kernel");
     return OB200_OK;
 }

@@ -23,6 +23,7 @@
 #pragma once
 #include "common.h"
 #include "internal.h"
+#include "packed_f32.cuh"
 #include "sm100_ptx.cuh"
 #include <atomic>
 #include <cuda_bf16.h>
@@ -99,40 +100,11 @@ __device__ __forceinline__ float team_max_nan(float v) {
     return v;
 }
 
-// Two fp32 in a register pair.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair(float a, float b) {
-    f32x2 v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
-__device__ __forceinline__ void halves(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 v;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
 __device__ __forceinline__ f32x2 ex2_2(f32x2 v) {
     float a, b;
     halves(v, a, b);
     return pair(ex2(a), ex2(b));
 }
-__device__ __forceinline__ float sum2(f32x2 v) {
-    float a, b;
-    halves(v, a, b);
-    return a + b;
-}
-
 // ---- 16 bytes of a row ------------------------------------------------------------
 // The value that stands for logits that do not count, and for those below it: in every element of a word, and as fp32.
 // A row whose largest logit is below half of it is worked on separately (careful_row).
@@ -581,7 +553,7 @@ __device__ __forceinline__ void copy_vectors(const PolicyRows& r, long long row,
 // ---- short rows --------------------------------------------------------------------
 // LANES lanes a row, 32 / LANES adjacent rows a warp; each warp has slots of its own and fills them itself.
 template <typename T, int KIND, int LANES, bool ALIKE>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(128, 6)
 policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {
     constexpr int R = 32 / LANES;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -701,28 +673,62 @@ __device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, vola
     return false;
 }
 
-// The last warp copies rows ahead, the others work on them; the first of those joins their sums, and the clusters'.
+// What a warp or a CTA found of a row, relative to its own largest logit m and reference logit c - or to 0 where it has no
+// ordinary one: its terms are 0 then.
+template <typename T>
+__device__ __forceinline__ float base_of(float top) { return top < Lowest<T>::kValue / 2 ? 0.f : top; }
+// Entries (m, c, s, t | a, b, za, -), one a lane, none in lanes from n on, as one.
+template <typename T, int KIND>
+__device__ __forceinline__ Sums join_entries(const float (*entry)[8], int n) {
+    const int lane = threadIdx.x % 32;
+    const float* mine = entry[lane < n ? lane : 0];
+    const float4 lo = *(const float4*)mine, hi = *(const float4*)(mine + 4);
+    Sums q;
+    q.m = warp_max_nan(lo.x);
+    q.c = KIND == kClippedRef ? warp_max_nan(lo.y) : 0.f;
+    q.za = KIND == kSearch ? 0.f : warp_max_nan(hi.z);
+    q.s = q.t = q.a = q.b = 0.f;
+    if (lane < n) {
+        const float d = base_of<T>(lo.x) - base_of<T>(q.m), f = lo.z == 0.f ? 0.f : ex2(d * kLog2e);
+        q.s = lo.z * f;
+        q.t = fmaf(d, q.s, lo.w * f);
+        if (KIND == kSearch) { q.a = fmaf(d, hi.y, hi.x); q.b = hi.y; }
+        if (KIND == kClippedRef) {
+            const float dc = base_of<T>(lo.y) - base_of<T>(q.c);
+            q.a = fmaf(d - dc, q.s, hi.x * f);
+            q.b = hi.y == 0.f ? 0.f : hi.y * ex2(dc * kLog2e);
+        }
+    }
+    q.s = team_sum(q.s); q.t = team_sum(q.t);
+    if (KIND != kClipped) { q.a = team_sum(q.a); q.b = team_sum(q.b); }
+    return q;
+}
+
+// Three kinds of warps that meet at barriers in shared memory only: the workers, which go over a row's vectors - the sums
+// of a row, then the gradient of the row before, whose sums have been joined meanwhile; one that joins the workers' sums
+// and the cluster's; one that copies rows ahead.
 template <typename T, int KIND, bool ALIKE>
 __global__ void __launch_bounds__(512, 2)
 policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {
     constexpr int V = 16 / sizeof(T);
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float top_of[2][16][2];
-    __shared__ float part[16][8];                // the warps' sums
-    __shared__ float joined[2][8][8];            // the cluster's CTAs' sums, by turns
-    __shared__ float found[12];                  // what comes of the row: RowGrad; live; apart
-    __shared__ __align__(8) unsigned long long full_bar[4], empty_bar[4], join_bar;
+    __shared__ __align__(16) float part[2][16][8];        // the workers' sums, by turns
+    __shared__ __align__(16) float joined[2][8][8];       // the cluster's CTAs' sums, by turns
+    __shared__ __align__(16) float found[2][12];          // what comes of a row: RowGrad; live; apart
+    __shared__ __align__(8) unsigned long long full_bar[4], empty_bar[4], sums_bar[2], found_bar[2], join_bar;
     __shared__ int abort_flag;
     uint32_t cta, ctas;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32 - 1, threads = 32 * warps;
-    const uint32_t smem_s = ptx::smem_u32(smem), full = ptx::smem_u32(full_bar), empty = ptx::smem_u32(empty_bar), join = ptx::smem_u32(&join_bar);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32 - 2, threads = 32 * warps;
+    const uint32_t smem_s = ptx::smem_u32(smem), full = ptx::smem_u32(full_bar), empty = ptx::smem_u32(empty_bar);
+    const uint32_t sums = ptx::smem_u32(sums_bar), ready = ptx::smem_u32(found_bar), join = ptx::smem_u32(&join_bar);
     if (threadIdx.x == 0) {
         for (int s = 0; s < sh.slots; ++s) {
-            ptx::mbar_init(full + 8 * s, 1 + (r.bits ? 32 : 0));
-            ptx::mbar_init(empty + 8 * s, warps);
+            ptx::mbar_init(full + 8 * s, 1 + (ALIKE && r.bits ? 32 : 0));
+            ptx::mbar_init(empty + 8 * s, warps + 1);
         }
+        for (int i = 0; i < 2; ++i) { ptx::mbar_init(sums + 8 * i, warps); ptx::mbar_init(ready + 8 * i, 1); }
         ptx::mbar_init(join, ctas);
         abort_flag = 0;
     }
@@ -732,17 +738,31 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
     if (ctas > 1) cluster_barrier();
     const int v0 = (int)cta * sh.seg;
     const long long first = blockIdx.x / ctas, step = gridDim.x / ctas;
-    int slot = 0;
+    // A wait that runs out is noted; the loops go on without waiting, so that every warp comes to its end.
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!ptx::mbar_wait_warp(bar, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+    };
+    auto part_of = [&](int slot) {
+        uint8_t* const at = smem + slot * sh.slot_bytes;
+        const int4 h = *(const int4*)(at + 16);
+        return Part{at + kHeader, at + sh.x_at, (const uint32_t*)(at + sh.mask_at), max(v0 * V - h.x, 0) >> 5, h.x, h.y,
+                    v0, min(h.y, v0 + sh.seg), (h.w & 1) != 0, (h.w & 2) != 0};
+    };
+    auto put_header = [&](int slot, float4 scalars, const Place& p) {
+        uint8_t* const at = smem + slot * sh.slot_bytes;
+        *(float4*)at = scalars;
+        *(int4*)(at + 16) = make_int4(p.head, p.vecs, 0, (p.first_out ? 1 : 0) | (p.last_out ? 2 : 0));
+    };
+    int slot = 0, turn = 0;                      // turn counts the rows that are not left out for their weight
     uint32_t parity = 0;
 
-    if (warp == warps) {
+    if (warp == warps + 1) {
         if (ALIKE) {
             float4 ahead = scalars_of(r, KIND, first);
             for (long long row = first; row < r.n; row += step) {
                 const float4 scalars = ahead;
                 ahead = scalars_of(r, KIND, row + step);
-                if (row >= first + sh.slots * step && !ptx::mbar_wait_warp(empty + 8 * slot, parity ^ 1, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
-                uint8_t* const at = smem + slot * sh.slot_bytes;
+                if (row >= first + sh.slots * step) wait(empty + 8 * slot, parity ^ 1);
                 const uint32_t at_s = smem_s + slot * sh.slot_bytes, bar = full + 8 * slot;
                 const Place p = place_of<T, KIND, ALIKE>(r, row);
                 const int v1 = min(p.vecs, v0 + sh.seg);
@@ -752,133 +772,85 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
                     arrive_after_copies(bar);
                 }
                 if (lane == 0) {
-                    *(float4*)at = scalars;
-                    *(int4*)(at + 16) = make_int4(p.head, p.vecs, 0, (p.first_out ? 1 : 0) | (p.last_out ? 2 : 0));
+                    put_header(slot, scalars, p);
                     copy_vectors<T, KIND>(r, row, p, v0, v1, at_s, sh.x_at, bar, scalars.x != 0.f);
                 }
                 __syncwarp();
                 if (++slot == sh.slots) { slot = 0; parity ^= 1; }
             }
-            if (abort_flag) {                    // a wait ran out: what is still in flight is waited for once more, within the same limit
+            if (abort_flag) {                    // what is still in flight is waited for once more, within the same limit
                 int none = 0;
                 for (int s = 0; s < sh.slots; ++s) ptx::mbar_wait(full + 8 * s, s >= slot ? parity ^ 1 : parity, &none);
             }
         }
-    } else {
-        int turn = 0;
-        uint32_t join_parity = 0;
+    } else if (warp == warps) {
         for (long long row = first; row < r.n; row += step) {
-            uint8_t* const at = smem + slot * sh.slot_bytes;
-            float4 scalars;
-            Place pl;
-            if (ALIKE) {
-                if (!ptx::mbar_wait_warp(full + 8 * slot, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
-                scalars = *(const float4*)at;
-                const int4 h = *(const int4*)(at + 16);
-                pl = Place{h.x, h.y, (h.w & 1) != 0, (h.w & 2) != 0};
+            wait(full + 8 * slot, parity);
+            const float4 scalars = *(const float4*)(smem + slot * sh.slot_bytes);
+            if (scalars.x == 0.f) {
+                if (lane == 0 && cta == 0) put_out(r, row, false, RowOut());
             } else {
-                scalars = scalars_of(r, KIND, row);
-                pl = place_of<T, KIND, ALIKE>(r, row);
-            }
-            const Part p{at + kHeader, at + sh.x_at, (const uint32_t*)(at + sh.mask_at), max(v0 * V - pl.head, 0) >> 5, pl.head, pl.vecs,
-                         v0, min(pl.vecs, v0 + sh.seg), pl.first_out, pl.last_out};
-            const float w = scalars.x;
-            if (!ALIKE) {
-                if (w != 0.f) copy_in<T, KIND>(r, row, p, threadIdx.x, threads);
-                named_sync(1, threads);
-            }
-            const int act = KIND == kSearch ? -1 : __float_as_int(scalars.w);
-            const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;   // the action's element of the row
-            bool live = w != 0.f, apart = false;
-            RowGrad g;
-            if (live) {                          // the same in the whole team
-                uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
-                pass_max<T, KIND, ALIKE>(r, row, p, threadIdx.x, threads, &top_z, &top_x);
-                Sums q;
-                q.m = warp_max_nan(word_top<T>(top_z));
-                q.c = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
-                if (lane == 0) { top_of[turn][warp][0] = q.m; top_of[turn][warp][1] = q.c; }
-                named_sync(1, threads);
-                const int i = lane < warps ? lane : 0;
-                q.m = warp_max_nan(top_of[turn][i][0]);
-                if (KIND == kClippedRef) q.c = warp_max_nan(top_of[turn][i][1]);
-                turn ^= 1;
-                const float top = q.m, top_ref = q.c;
-                // a part without an ordinary logit: its terms vanish next to 0
-                if (q.m < Lowest<T>::kValue / 2) q.m = 0.f;
-                if (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2) q.c = 0.f;
-                pass_sums<T, KIND>(p, threadIdx.x, threads, q);
-                q.s = team_sum(q.s);
-                q.t = team_sum(q.t);
-                if (KIND != kClipped) { q.a = team_sum(q.a); q.b = team_sum(q.b); }
-                if (lane == 0) {
-                    *(float4*)part[warp] = make_float4(q.s, q.t, q.a, q.b);
-                }
-                if (warp != 0) {
-                    named_arrive(2, threads);
-                } else {
-                    named_sync(2, threads);
-                    float4 v = lane < warps ? *(const float4*)part[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    q.s = team_sum<16>(v.x); q.t = team_sum<16>(v.y);
-                    if (KIND != kClipped) { q.a = team_sum<16>(v.z); q.b = team_sum<16>(v.w); }
-                    q.za = -kInf;
-                    if (KIND != kSearch && act_e >= 0 && act_e / V >= v0 && act_e / V < p.v1 &&
+                const int by = turn & 1;
+                wait(sums + 8 * by, (turn >> 1) & 1);
+                Sums q = join_entries<T, KIND>(part[by], warps);
+                q.za = -kInf;
+                if (KIND != kSearch) {
+                    const Part p = part_of(slot);
+                    const int act = __float_as_int(scalars.w), e = act + p.head;
+                    if ((unsigned)act < (unsigned)r.A && e / V >= v0 && e / V < p.v1 &&
                         (!r.bits || (p.ms[(act >> 5) - p.mask_first] >> (act & 31)) & 1u))
-                        q.za = to_f32(((const T*)p.zs)[act_e - v0 * V]);
-                    float M = top, C = top_ref;
-                    if (ctas > 1) {
-                        // its sums to every CTA of the cluster, and theirs relative to the largest maxima
-                        float (*all)[8] = joined[join_parity];
-                        if (lane < (int)ctas) {
-                            uint32_t there, bar;
-                            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(ptx::smem_u32(all[cta])), "r"(lane));
-                            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(join), "r"(lane));
-                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(top), "f"(top_ref), "f"(q.s), "f"(q.t) : "memory");
-                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + 16), "f"(q.a), "f"(q.b), "f"(q.za), "f"(0.f) : "memory");
-                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-                        }
-                        if (!__all_sync(~0u, cluster_wait(join, join_parity, &abort_flag))) { abort_flag = 1; atomicExch(sh.error, 4); }
-                        join_parity ^= 1;
-                        const float* mine = all[lane < (int)ctas ? lane : 0];
-                        const float4 lo = *(const float4*)mine, hi = *(const float4*)(mine + 4);
-                        M = warp_max_nan(lo.x);
-                        C = KIND == kClippedRef ? warp_max_nan(lo.y) : 0.f;
-                        q.za = warp_max_nan(hi.z);
-                        q.s = q.t = q.a = q.b = 0.f;
-                        if (lane < (int)ctas) {
-                            const float m = lo.x < Lowest<T>::kValue / 2 ? 0.f : lo.x, c = lo.y < Lowest<T>::kValue / 2 ? 0.f : lo.y;
-                            const float d = m - M, dc = c - C, f = lo.z == 0.f ? 0.f : ex2(d * kLog2e);
-                            q.s = lo.z * f;
-                            q.t = fmaf(d, q.s, lo.w * f);
-                            if (KIND == kSearch) { q.a = fmaf(d, hi.y, hi.x); q.b = hi.y; }
-                            if (KIND == kClippedRef) { q.a = fmaf(d - dc, q.s, hi.x * f); q.b = hi.y == 0.f ? 0.f : hi.y * ex2(dc * kLog2e); }
-                        }
-                        q.s = team_sum<8>(q.s); q.t = team_sum<8>(q.t);
-                        if (KIND != kClipped) { q.a = team_sum<8>(q.a); q.b = team_sum<8>(q.b); }
-                    }
-                    q.m = M; q.c = C;
-                    apart = M < Lowest<T>::kValue / 2 || (KIND == kClippedRef && C < Lowest<T>::kValue / 2);
-                    RowOut out;
-                    live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out);
-                    if (apart) {
-                        if (cta == 0) careful_row<T, KIND>(r, row);
-                    } else if (lane == 0 && cta == 0) {
-                        put_out(r, row, live, out);
-                    }
-                    if (lane == 0) {
-                        *(float4*)found = make_float4(g.M, g.C, g.lp, g.k0);
-                        *(float4*)(found + 4) = make_float4(g.kz, g.kd, g.ka, g.kt);
-                        found[8] = live ? 1.f : 0.f;
-                        found[9] = apart ? 1.f : 0.f;
-                    }
+                        q.za = to_f32(((const T*)p.zs)[e - v0 * V]);
                 }
-                named_sync(3, threads);
-                const float4 lo = *(const float4*)found, hi = *(const float4*)(found + 4);
+                if (ctas > 1) {
+                    // its sums to every CTA of the cluster
+                    if (lane < (int)ctas) {
+                        uint32_t there, bar;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(ptx::smem_u32(joined[by][cta])), "r"(lane));
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(join), "r"(lane));
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(q.m), "f"(q.c), "f"(q.s), "f"(q.t) : "memory");
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + 16), "f"(q.a), "f"(q.b), "f"(q.za), "f"(0.f) : "memory");
+                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+                    }
+                    if (!__all_sync(~0u, cluster_wait(join, turn & 1, &abort_flag))) { abort_flag = 1; atomicExch(sh.error, 4); }
+                    q = join_entries<T, KIND>(joined[by], (int)ctas);
+                }
+                const bool apart = q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2);
+                RowGrad g;
+                RowOut out;
+                const bool live = row_result<KIND>(r, q, scalars.x, scalars.y, scalars.z, &g, &out);
+                if (lane == 0) {
+                    *(float4*)found[by] = make_float4(g.M, g.C, g.lp, g.k0);
+                    *(float4*)(found[by] + 4) = make_float4(g.kz, g.kd, g.ka, g.kt);
+                    found[by][8] = live ? 1.f : 0.f;
+                    found[by][9] = apart ? 1.f : 0.f;
+                    ptx::mbar_arrive(ready + 8 * by);
+                    if (cta == 0 && !apart) put_out(r, row, live, out);
+                }
+                __syncwarp();
+                if (apart && cta == 0) careful_row<T, KIND>(r, row);
+                ++turn;
+            }
+            if (lane == 0) ptx::mbar_arrive(empty + 8 * slot);
+            if (++slot == sh.slots) { slot = 0; parity ^= 1; }
+        }
+    } else {
+        // The gradient of a row whose sums are on their way.
+        auto finish = [&](long long row, int s, int by) {          // by: its turn, -1 when it is left out for its weight
+            const Part p = part_of(s);
+            RowGrad g;
+            bool live = false, apart = false;
+            int act_e = -1;
+            if (by >= 0) {
+                wait(ready + 8 * (by & 1), (by >> 1) & 1);
+                const float* f = found[by & 1];
+                const float4 lo = *(const float4*)f, hi = *(const float4*)(f + 4);
                 g = RowGrad{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                live = found[8] != 0.f;
-                apart = found[9] != 0.f;
-            } else if (threadIdx.x == 0 && cta == 0) {
-                put_out(r, row, false, RowOut());
+                live = f[8] != 0.f;
+                apart = f[9] != 0.f;
+                if (KIND != kSearch) {
+                    const int act = __float_as_int(((const float*)(smem + s * sh.slot_bytes))[3]);
+                    if ((unsigned)act < (unsigned)r.A) act_e = act + p.head;
+                }
             }
             T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
             if (!apart) pass_grad<T, KIND, ALIKE>(r, p, threadIdx.x, threads, live, g, act_e, grad);
@@ -886,14 +858,54 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
                 // the slot's next copy comes behind what was read and written here
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(empty + 8 * slot);
+                if (lane == 0) ptx::mbar_arrive(empty + 8 * s);
             } else {
                 named_sync(1, threads);
                 if (!apart) copy_out<T>(r, p, threadIdx.x, threads, grad);
-                named_sync(1, threads);
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(empty + 8 * s);
             }
+        };
+        int before = -1, before_turn = -1;       // slot and turn of the row that is to be finished
+        for (long long row = first; row < r.n; row += step) {
+            if (!ALIKE) {
+                const float4 scalars = scalars_of(r, KIND, row);
+                const Place pl = place_of<T, KIND, ALIKE>(r, row);
+                if (row >= first + sh.slots * step) wait(empty + 8 * slot, parity ^ 1);
+                if (threadIdx.x == 0) put_header(slot, scalars, pl);
+                named_sync(1, threads);
+                if (scalars.x != 0.f) copy_in<T, KIND>(r, row, part_of(slot), threadIdx.x, threads);
+                named_sync(1, threads);
+                if (threadIdx.x == 0) ptx::mbar_arrive(full + 8 * slot);
+            }
+            wait(full + 8 * slot, parity);
+            const bool live = *(const float*)(smem + slot * sh.slot_bytes) != 0.f;
+            if (live) {
+                const Part p = part_of(slot);
+                uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
+                pass_max<T, KIND, ALIKE>(r, row, p, threadIdx.x, threads, &top_z, &top_x);
+                const float top = warp_max_nan(word_top<T>(top_z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
+                Sums q;
+                q.m = base_of<T>(top);
+                q.c = KIND == kClippedRef ? base_of<T>(top_ref) : 0.f;
+                pass_sums<T, KIND>(p, threadIdx.x, threads, q);
+                q.s = team_sum(q.s);
+                q.t = team_sum(q.t);
+                if (KIND != kClipped) { q.a = team_sum(q.a); q.b = team_sum(q.b); }
+                if (lane == 0) {
+                    float* to = part[turn & 1][warp];
+                    *(float4*)to = make_float4(top, top_ref, q.s, q.t);
+                    *(float4*)(to + 4) = make_float4(q.a, q.b, 0.f, 0.f);
+                }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(sums + 8 * (turn & 1));
+            }
+            if (before >= 0) finish(row - step, before, before_turn);
+            before = slot;
+            before_turn = live ? turn++ : -1;
             if (++slot == sh.slots) { slot = 0; parity ^= 1; }
         }
+        if (before >= 0) finish(first + (r.n - 1 - first) / step * step, before, before_turn);
     }
     __syncwarp();
     // and none may leave while another may still write
@@ -933,7 +945,7 @@ int launch_warp_rows(const PolicyRows& r, const RowShape& sh, cudaStream_t st) {
     auto kernel = policy_warp_rows_kernel<T, KIND, LANES, ALIKE>;
     int facts;
     if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
-    const int warp_bytes = sh.slots * (R * sh.slot_bytes + 16), fit = 104 * 1024 / warp_bytes, warps = fit < 1 ? 1 : fit > 8 ? 8 : fit;
+    const int warp_bytes = sh.slots * (R * sh.slot_bytes + 16), fit = 104 * 1024 / warp_bytes, warps = fit < 1 ? 1 : fit > 4 ? 4 : fit;
     const long long teams = ((long long)r.n + R * warps - 1) / (R * warps), room = resident_ctas(facts, 32 * warps, warps * warp_bytes);
     kernel<<<(unsigned)(teams < room ? teams : room), 32 * warps, warps * warp_bytes, st>>>(r, sh);
     OB200_LAUNCHED("policy_warp_rows_kernel");
@@ -946,7 +958,7 @@ int launch_cta_rows(const PolicyRows& r, const RowShape& sh, int warps, int ctas
     auto kernel = policy_cta_rows_kernel<T, KIND, ALIKE>;
     int facts;
     if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
-    const int threads = 32 * (warps + 1), smem = sh.slots * sh.slot_bytes;
+    const int threads = 32 * (warps + 2), smem = sh.slots * sh.slot_bytes;
     const long long room = resident_ctas(facts, threads, smem) / ctas;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -976,18 +988,19 @@ int launch_shape(const PolicyRows& r, cudaStream_t st) {
     };
     if (r.A <= 1024) {
         lay(1);
-        sh.slots = 2;
-        if (ALIKE && sh.slot_bytes <= 2400) return launch_warp_rows<T, KIND, ALIKE ? 8 : 32, ALIKE>(r, sh, st);
-        if (ALIKE && sh.slot_bytes <= 4800) return launch_warp_rows<T, KIND, ALIKE ? 16 : 32, ALIKE>(r, sh, st);
+        sh.slots = 1;
+        if (ALIKE && sh.slot_bytes <= 2400 && r.n > 8192) return launch_warp_rows<T, KIND, ALIKE ? 8 : 32, ALIKE>(r, sh, st);
+        if (ALIKE && sh.slot_bytes <= 4800 && r.n > 4096) return launch_warp_rows<T, KIND, ALIKE ? 16 : 32, ALIKE>(r, sh, st);
         return launch_warp_rows<T, KIND, 32, ALIKE>(r, sh, st);
     }
     if ((long long)vecs * (16 + XV) <= 8LL * kMostShared / 2) {
         int ctas = 1;
-        while (ctas < 8 && lay(ctas) > 36 * 1024) ctas *= 2;
+        int most = 36 * 1024;
+        while (ctas < 8 && lay(ctas) > most) ctas *= 2;
         if (2 * lay(ctas) <= kMostShared) {
-            sh.slots = 2;
-            const int warps = (sh.seg + 191) / 192;
-            return launch_cta_rows<T, KIND, ALIKE>(r, sh, warps < 2 ? 2 : warps > 15 ? 15 : warps, ctas, st);
+            sh.slots = 3 * sh.slot_bytes <= kMostShared ? 3 : 2;
+            const int warps = (sh.seg + 95) / 96;
+            return launch_cta_rows<T, KIND, ALIKE>(r, sh, warps < 2 ? 2 : warps > 14 ? 14 : warps, ctas, st);
         }
     }
     policy_long_rows_kernel<T, KIND><<<(unsigned)r.n, 512, 0, st>>>(r);

@@ -191,8 +191,10 @@ def test_adamw_8_codes_are_exact(api, p_dt, g_dt, shift):
             g = opt.grads[i].float()
             m = dequantise(st["exp_avg"][i], st["exp_avg_scale"][i])
             v = dequantise(st["exp_avg_sq"][i], st["exp_avg_sq_scale"][i]).square()
-            m = m * 0.9 + g * (1.0 - 0.9)
-            v = v * 0.999 + (g * g) * (1.0 - 0.999)
+            # fused multiply-adds: in 64 bits the product is exact, and the sum's second rounding moves none of these values
+            b1, b2 = float(np.float32(0.9)), float(np.float32(0.999))
+            m = (m.double() * b1 + (g * (1.0 - 0.9)).double()).float()
+            v = (v.double() * b2 + ((g * g) * (1.0 - 0.999)).double()).float()
             mq, msc = quantise(m, False)
             vq, vsc = quantise(v.sqrt(), True)
             assert torch.equal(opt.state["exp_avg_scale"][i], msc) and torch.equal(opt.state["exp_avg_sq_scale"][i], vsc), i
