@@ -92,6 +92,16 @@ __device__ __forceinline__ float team_sum(float v) {
     for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     return v;
 }
+// Four sums over the warp in 6 exchanges instead of 20: lane i ends with the sum of the (i mod 4)th.
+__device__ __forceinline__ float four_sums(float s, float t, float a, float b) {
+    const int lane = threadIdx.x % 32;
+    const bool odd = lane & 1, high = lane & 2;
+    const float u = (odd ? t : s) + __shfl_xor_sync(~0u, odd ? s : t, 1), v = (odd ? b : a) + __shfl_xor_sync(~0u, odd ? a : b, 1);
+    float w = (high ? v : u) + __shfl_xor_sync(~0u, high ? u : v, 2);
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) w += __shfl_xor_sync(~0u, w, o);
+    return w;
+}
 template <int LANES = 32>
 __device__ __forceinline__ float team_max_nan(float v) {
     if (LANES == 32) return warp_max_nan(v);
@@ -121,6 +131,17 @@ __device__ __forceinline__ f32x2 elements(const uint32_t* v, int i) {
     const float2 f = __half22float2(*(const __half2*)&v[i]);
     return pair(f.x, f.y);
 }
+// The same less c (given as -c), in fp32: a 16-bit operand needs no conversion of its own.
+template <typename T>
+__device__ __forceinline__ f32x2 elements_less(const uint32_t* v, int i, f32x2 minus_c, float c) {
+    if (sizeof(T) == 4) return add2(elements<T>(v, i), minus_c);
+    float a, b;
+    if (std::is_same<T, __nv_bfloat16>::value)
+        asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; sub.rn.f32.bf16 %0, l, %3; sub.rn.f32.bf16 %1, h, %3;}" : "=f"(a), "=f"(b) : "r"(v[i]), "f"(c));
+    else
+        asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; sub.rn.f32.f16 %0, l, %3; sub.rn.f32.f16 %1, h, %3;}" : "=f"(a), "=f"(b) : "r"(v[i]), "f"(c));
+    return pair(a, b);
+}
 // The larger values of two words, element by element, NaN where either is.
 template <typename T>
 __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b) {
@@ -147,20 +168,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *(const uint32_t*)&v;
 }
-// Masks of the elements of a vector whose bits in `on` are set, word by word.
-template <typename T>
+// Masks of the eight 16-bit elements of a vector whose bits in `on` are set, word by word.
 __device__ __forceinline__ void word_masks(uint32_t on, uint32_t (&m)[4]) {
-    if (sizeof(T) == 4) {
+    // four bits to the signs of four bytes, each sign over a half word
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m[i] = (on >> i) & 1u ? ~0u : 0u;
-    } else {
-        // four bits to the signs of four bytes, each sign over a half word
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t signs = ((on >> (4 * i)) & 15u) * 0x10204080u;
-            asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m[2 * i]) : "r"(signs));
-            asm("prmt.b32 %0, %1, 0, 0xBBAA;" : "=r"(m[2 * i + 1]) : "r"(signs));
-        }
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t signs = ((on >> (4 * i)) & 15u) * 0x10204080u;
+        asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m[2 * i]) : "r"(signs));
+        asm("prmt.b32 %0, %1, 0, 0xBBAA;" : "=r"(m[2 * i + 1]) : "r"(signs));
     }
 }
 __device__ __forceinline__ void load16(const uint8_t* p, uint32_t* to) {
@@ -184,7 +199,7 @@ __device__ __forceinline__ bool row_result(const PolicyRows& r, const Sums& q, f
     g->M = q.m; g->C = q.c; g->lp = -l2s;
     g->kz = w * r.entropy; g->kd = 0.f; g->ka = 0.f; g->kt = 0.f;
     if (KIND == kSearch) {
-        const float inv_T = 1.f / q.b, ce = fmaf(-q.a, inv_T, ls);
+        const float inv_T = __fdividef(1.f, q.b), ce = fmaf(-q.a, inv_T, ls);
         g->k0 = w * (1.f - r.entropy * mean);
         g->kt = w * inv_T;
         o->loss = w * (ce - r.entropy * H);
@@ -231,7 +246,7 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
     auto second = [&](int j) { return KIND == kSearch ? target_f32(((const uint32_t*)x)[j], r.visits) : KIND == kClippedRef ? to_f32(((const T*)x)[j]) : 0.f; };
     Sums q{-kInf, -kInf, 0.f, 0.f, 0.f, 0.f, -kInf};
     bool live = w != 0.f;
-    if (live && bits) {                          // most rows that come here have no legal action
+    if (live && bits) {
         float some = 0.f;
         for (int i = tid; i < (r.A + 31) / 32; i += threads)
             if (bits[i] & (i == r.A / 32 ? ~(~0u << (r.A & 31)) : ~0u)) some = 1.f;
@@ -280,7 +295,7 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
     }
 }
 
-// Rows without an ordinary logit - no legal action, or all of them at a type's lowest value or -inf - by one warp.
+// Rows without an ordinary logit - all of them at a type's lowest value or -inf - by one warp.
 template <typename T, int KIND>
 __device__ __noinline__ void careful_row(const PolicyRows& r, long long row) {
     plain_row<T, KIND>(r, row, threadIdx.x % 32, 32, [](float v, bool is_max) { return is_max ? warp_max_nan(v) : team_sum(v); });
@@ -307,7 +322,6 @@ policy_long_rows_kernel(const __grid_constant__ PolicyRows r) {
 struct RowShape {
     int seg;                            // vectors a CTA holds of a row
     int x_at, mask_at, slot_bytes;      // offsets in a slot, its size
-    int slots;                          // slots in turn
     int* error;
 };
 constexpr int kHeader = 32;             // weight, old log-probability, advantage, action; head, vectors, -, flags
@@ -348,156 +362,353 @@ struct Part {
     bool first_out, last_out;
 };
 
-// First pass, over vectors v0 + tid, + stride ...: the largest words; what does not count becomes the lowest value (a target
-// 0), visit counts become fp32.
-template <typename T, int KIND, bool ALIKE>
-__device__ __forceinline__ void pass_max(const PolicyRows& r, long long row, const Part& p, int tid, int stride, uint32_t* top_z, uint32_t* top_x) {
-    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
-    constexpr uint32_t kLowWord = Lowest<T>::kWord;
-    const int edge_first = p.head ? 0 : -1, edge_last = (p.head + r.A) % V ? p.vecs - 1 : -1;
-    for (int v = p.v0 + tid; v < p.v1; v += stride) {
-        uint8_t *zp = p.zs + (v - p.v0) * 16, *xp = p.xs + (v - p.v0) * XV;
-        uint32_t z[4], x[XV / 4];
-        load16(zp, z);
-        const bool edge = v == edge_first || v == edge_last;
-        if (KIND == kClippedRef || (KIND == kSearch && (r.bits || r.visits || edge)))
+// The words of vector v of a part.
+template <typename T, int KIND>
+struct Vec {
+    static constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XW = KIND == kClipped ? 1 : V * XB / 4;
+    uint32_t z[4], x[XW];
+    __device__ __forceinline__ void load_z(const Part& p, int v) { load16(p.zs + (v - p.v0) * 16, z); }
+    __device__ __forceinline__ void load_x(const Part& p, int v) {
+        if (KIND != kClipped)
 #pragma unroll
-            for (int i = 0; i < XV / 16; ++i) load16(xp + 16 * i, x + 4 * i);
-        if (r.bits || edge) {
-            const int j = v * V - p.head;                   // the first element's action; below 0 in the first vector
-            if (ALIKE && ((v == 0 && p.first_out) || (v == p.vecs - 1 && p.last_out))) {
-                // not copied: it reaches beyond the matrix
-                for (int i = 0; i < V; ++i)
-                    if (j + i >= 0 && j + i < r.A) {
-                        ((T*)zp)[i] = ((const T*)r.z)[row * r.z_pitch + j + i];
-                        if (KIND == kSearch) ((uint32_t*)xp)[i] = ((const uint32_t*)r.x)[row * r.x_pitch + j + i];
-                        if (KIND == kClippedRef) ((T*)xp)[i] = ((const T*)r.x)[row * r.x_pitch + j + i];
-                    }
-                load16(zp, z);
-                if (KIND != kClipped)
+            for (int i = 0; i < XW / 4; ++i) load16(p.xs + (v - p.v0) * (XW * 4) + 16 * i, x + 4 * i);
+    }
+    __device__ __forceinline__ void store_z(const Part& p, int v) const { store16(p.zs + (v - p.v0) * 16, z); }
+    __device__ __forceinline__ void store_x(const Part& p, int v) const {
+        if (KIND != kClipped)
 #pragma unroll
-                    for (int i = 0; i < XV / 16; ++i) load16(xp + 16 * i, x + 4 * i);
-            }
-            uint32_t on = ~0u;
-            if (r.bits) {
-                const int i = (j >> 5) - p.mask_first, most = (r.A - 1) >> 5;
-                const uint32_t lo = j < 0 ? 0u : p.ms[i], hi = (j & 31) + V > 32 && (j >> 5) < most ? p.ms[i + 1] : 0u;
-                on = __funnelshift_r(lo, hi, j & 31);
-            }
-            if (j < 0) on &= ~0u << -j;
-            if (j + V > r.A) on &= ~(~0u << (r.A - j));
-            uint32_t m[4];
-            word_masks<T>(on, m);
+            for (int i = 0; i < XW / 4; ++i) store16(p.xs + (v - p.v0) * (XW * 4) + 16 * i, x + 4 * i);
+    }
+    // Elements without their bit in `on` become the lowest value, their targets 0.
+    __device__ __forceinline__ void keep(uint32_t on) {
+        if (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                z[i] = (z[i] & m[i]) | (kLowWord & ~m[i]);
-                if (KIND == kClippedRef) x[i] = (x[i] & m[i]) | (kLowWord & ~m[i]);
+                const bool is = on & (1u << i);
+                z[i] = is ? z[i] : Lowest<T>::kWord;
+                if (KIND == kClippedRef) x[i % XW] = is ? x[i % XW] : Lowest<T>::kWord;
+                if (KIND == kSearch) x[i % XW] = is ? x[i % XW] : 0u;
+            }
+        } else {
+            uint32_t m[4];
+            word_masks(on, m);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                z[i] = (z[i] & m[i]) | (Lowest<T>::kWord & ~m[i]);
+                if (KIND == kClippedRef) x[i % XW] = (x[i % XW] & m[i]) | (Lowest<T>::kWord & ~m[i]);
             }
             if (KIND == kSearch)
 #pragma unroll
-                for (int i = 0; i < V; ++i) x[i] = (on >> i) & 1u ? x[i] : 0u;
+                for (int i = 0; i < V; ++i) x[i % XW] = on & (1u << i) ? x[i % XW] : 0u;
         }
-        if (KIND == kSearch && (r.bits || r.visits || edge)) {
-            if (r.visits)
+    }
+    __device__ __forceinline__ void counts_to_f32() {
 #pragma unroll
-                for (int i = 0; i < V; ++i) x[i] = __float_as_uint((float)(int)x[i]);
-#pragma unroll
-            for (int i = 0; i < XV / 16; ++i) store16(xp + 16 * i, x + 4 * i);
-        }
+        for (int i = 0; i < XW; ++i) x[i] = __float_as_uint((float)(int)x[i]);
+    }
+    // Not below the lowest value; the largest words.
+    __device__ __forceinline__ void raise(uint32_t* top_z, uint32_t* top_x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            z[i] = word_max<T>(z[i], kLowWord);
+            z[i] = word_max<T>(z[i], Lowest<T>::kWord);
             *top_z = word_max<T>(*top_z, z[i]);
             if (KIND == kClippedRef) {
-                x[i] = word_max<T>(x[i], kLowWord);
-                *top_x = word_max<T>(*top_x, x[i]);
+                x[i % XW] = word_max<T>(x[i % XW], Lowest<T>::kWord);
+                *top_x = word_max<T>(*top_x, x[i % XW]);
             }
         }
-        store16(zp, z);
-        if (KIND == kClippedRef) store16(xp, x);
     }
+};
+
+// Vectors of a part that lie in the row as a whole: [lo, hi); the outer ones, or -1.
+struct Inner { int lo, hi, first, last; };
+template <int V>
+__device__ __forceinline__ Inner inner_of(const PolicyRows& r, const Part& p) {
+    const bool head = p.head != 0, tail = ((p.head + r.A) & (V - 1)) != 0;
+    Inner n{p.v0, p.v1, -1, -1};
+    if (head && p.v0 == 0 && p.v1 > 0) { n.first = 0; n.lo = 1; }
+    if (tail && p.v1 == p.vecs && p.v1 > n.lo) { n.last = p.vecs - 1; n.hi = p.v1 - 1; }
+    return n;
+}
+
+// Bits of the legal actions of vector v; a vector that starts ahead of the row, or ends behind it, has none there.
+template <int V>
+__device__ __forceinline__ uint32_t bits_of(const PolicyRows& r, const Part& p, int v) {
+    const int j = v * V - p.head;                           // the first element's action; below 0 in the first vector
+    uint32_t on = ~0u;
+    if (r.bits) {
+        const int i = (j >> 5) - p.mask_first, most = (r.A - 1) >> 5;
+        const uint32_t lo = j < 0 ? 0u : p.ms[i], hi = (j & 31) + V > 32 && (j >> 5) < most ? p.ms[i + 1] : 0u;
+        on = __funnelshift_r(lo, hi, j & 31);
+    }
+    if (j < 0) on &= ~0u << -j;
+    if (j + V > r.A) on &= ~(~0u << (r.A - j));
+    return on;
+}
+
+// An outer vector that was not copied, because it reaches beyond the matrix, element by element.
+template <typename T, int KIND>
+__device__ __noinline__ void fetch_vector(const PolicyRows& r, long long row, const Part& p, int v) {
+    constexpr int V = 16 / sizeof(T);
+    const int j = v * V - p.head, at = (v - p.v0) * V;
+    for (int i = 0; i < V; ++i)
+        if (j + i >= 0 && j + i < r.A) {
+            ((T*)p.zs)[at + i] = ((const T*)r.z)[row * r.z_pitch + j + i];
+            if (KIND == kSearch) ((uint32_t*)p.xs)[at + i] = ((const uint32_t*)r.x)[row * r.x_pitch + j + i];
+            if (KIND == kClippedRef) ((T*)p.xs)[at + i] = ((const T*)r.x)[row * r.x_pitch + j + i];
+        }
+}
+
+// First pass, over vectors v0 + tid, + stride ...: the largest words; what does not count becomes the lowest value (a target
+// 0), visit counts become fp32.  Returns whether any action met was legal.
+// SHORT: rows of a few vectors a thread take their outer vectors along in the loop; the others' loops are free of them.
+template <typename T, int KIND, bool ALIKE, int U, bool SHORT>
+__device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, const Part& p, int tid, int stride, uint32_t* top_z, uint32_t* top_x) {
+    constexpr int V = 16 / sizeof(T);
+    uint32_t any = r.bits ? 0u : ~0u;
+    using W = Vec<T, KIND>;
+    const Inner n = inner_of<V>(r, p);
+    int v = p.v0 + tid;
+    if (SHORT) {
+        if (ALIKE && (p.first_out || p.last_out)) {
+            if (p.first_out && tid == 0 && p.v1 > 0) fetch_vector<T, KIND>(r, row, p, 0);
+            if (p.last_out && p.v1 > 0 && (p.vecs - 1) % stride == tid) fetch_vector<T, KIND>(r, row, p, p.vecs - 1);
+        }
+        for (; v < p.v1; v += stride) {
+            W w;
+            w.load_z(p, v);
+            const bool edge = v == n.first || v == n.last, change = r.bits || edge;
+            if (KIND == kClippedRef || (KIND == kSearch && (change || r.visits))) w.load_x(p, v);
+            if (change) {
+                const uint32_t on = bits_of<V>(r, p, v);
+                any |= on & ((1u << V) - 1);
+                w.keep(on);
+            }
+            if (KIND == kSearch && r.visits) w.counts_to_f32();
+            w.raise(top_z, top_x);
+            w.store_z(p, v);
+            if (KIND == kClippedRef || (KIND == kSearch && (change || r.visits))) w.store_x(p, v);
+        }
+        return any != 0u;
+    }
+    if (v < n.lo) v += stride;
+    if (r.bits) {
+        for (; v < n.hi; v += stride) {
+            W w;
+            w.load_z(p, v);
+            w.load_x(p, v);
+            const int j = v * V - p.head, i = (j >> 5) - p.mask_first;
+            uint32_t on = p.ms[i] >> (j & 31);
+            if ((j & 31) + V > 32) on |= p.ms[i + 1] << (32 - (j & 31));
+            any |= on & ((1u << V) - 1);
+            w.keep(on);
+            if (KIND == kSearch) {
+                if (r.visits) w.counts_to_f32();
+                w.store_x(p, v);
+            }
+            w.raise(top_z, top_x);
+            w.store_z(p, v);
+            if (KIND == kClippedRef) w.store_x(p, v);
+        }
+    } else if (KIND == kSearch && r.visits) {
+        for (; v < n.hi; v += stride) {
+            W w;
+            w.load_z(p, v);
+            w.load_x(p, v);
+            w.counts_to_f32();
+            w.store_x(p, v);
+            w.raise(top_z, top_x);
+            w.store_z(p, v);
+        }
+    } else {
+        for (; v + (U - 1) * stride < n.hi; v += U * stride) {
+            W w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                w[u].load_z(p, v + u * stride);
+                if (KIND == kClippedRef) w[u].load_x(p, v + u * stride);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                w[u].raise(top_z, top_x);
+                w[u].store_z(p, v + u * stride);
+                if (KIND == kClippedRef) w[u].store_x(p, v + u * stride);
+            }
+        }
+        for (; v < n.hi; v += stride) {
+            W w;
+            w.load_z(p, v);
+            if (KIND == kClippedRef) w.load_x(p, v);
+            w.raise(top_z, top_x);
+            w.store_z(p, v);
+            if (KIND == kClippedRef) w.store_x(p, v);
+        }
+    }
+    for (int k = 0; k < 2; ++k) {
+        // the first vector is thread 0's; the last one's thread has come to it by its steps
+        const int e = k ? n.last : n.first;
+        if (e < 0 || (k ? v != e : tid != 0)) continue;
+        if (ALIKE && ((e == 0 && p.first_out) || (e == p.vecs - 1 && p.last_out))) fetch_vector<T, KIND>(r, row, p, e);
+        W w;
+        w.load_z(p, e);
+        w.load_x(p, e);
+        const uint32_t on = bits_of<V>(r, p, e);
+        any |= on & ((1u << V) - 1);
+        w.keep(on);
+        if (KIND == kSearch && r.visits) w.counts_to_f32();
+        w.raise(top_z, top_x);
+        w.store_z(p, e);
+        w.store_x(p, e);
+    }
+    return any != 0u;
 }
 
 // Second pass: the sums relative to q.m and q.c.
-template <typename T, int KIND>
+template <typename T, int KIND, int U>
 __device__ __forceinline__ void pass_sums(const Part& p, int tid, int stride, Sums& q) {
-    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
+    constexpr int V = 16 / sizeof(T);
+    using W = Vec<T, KIND>;
     const f32x2 M = pair(-q.m, -q.m), C = pair(-q.c, -q.c), L = pair(kLog2e, kLog2e), minus = pair(-1.f, -1.f);
     f32x2 s = 0, t = 0, a = 0, b = 0;
-#pragma unroll 2
-    for (int v = p.v0 + tid; v < p.v1; v += stride) {
-        uint32_t z[4], x[XV / 4];
-        load16(p.zs + (v - p.v0) * 16, z);
-        if (KIND != kClipped)
-#pragma unroll
-            for (int i = 0; i < XV / 16; ++i) load16(p.xs + (v - p.v0) * XV + 16 * i, x + 4 * i);
+    auto add = [&](const W& w) {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
-            const f32x2 d = add2(elements<T>(z, i), M), e = ex2_2(mul2(d, L));
+            const f32x2 d = elements_less<T>(w.z, i, M, q.m), e = ex2_2(mul2(d, L));
             s = add2(s, e);
             t = fma2(e, d, t);
             if (KIND == kSearch) {
-                const f32x2 y = elements<float>(x, i);
+                const f32x2 y = elements<float>(w.x, i);
                 a = fma2(y, d, a);
                 b = add2(b, y);
             }
             if (KIND == kClippedRef) {
-                const f32x2 c = add2(elements<T>(x, i), C);
+                const f32x2 c = elements_less<T>(w.x, i, C, q.c);
                 b = add2(b, ex2_2(mul2(c, L)));
                 a = fma2(e, fma2(c, minus, d), a);
             }
         }
+    };
+    int v = p.v0 + tid;
+    for (; v + (U - 1) * stride < p.v1; v += U * stride) {
+        W w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) { w[u].load_z(p, v + u * stride); w[u].load_x(p, v + u * stride); }
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(w[u]);
+    }
+    for (; v < p.v1; v += stride) {
+        W w;
+        w.load_z(p, v);
+        w.load_x(p, v);
+        add(w);
     }
     q.s = sum2(s); q.t = sum2(t); q.a = sum2(a); q.b = sum2(b);
 }
 
 // Third pass: the gradient (0 where the row is not live), to `grad` (the row's element 0 stands at grad + head), or into
 // the slot where stores of vectors are not possible.
-template <typename T, int KIND, bool ALIKE>
+template <typename T, int KIND, bool ALIKE, int U, bool SHORT>
 __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, int tid, int stride, bool live, const RowGrad& g, int act_e, T* grad) {
-    constexpr int V = 16 / sizeof(T), XB = KIND == kSearch ? 4 : (int)sizeof(T), XV = V * XB;
+    constexpr int V = 16 / sizeof(T);
+    using W = Vec<T, KIND>;
     const f32x2 M = pair(-g.M, -g.M), C = pair(-g.C, -g.C), L = pair(kLog2e, kLog2e), minus = pair(-1.f, -1.f);
     const f32x2 lp = pair(g.lp, g.lp), k0 = pair(g.k0, g.k0), kz = pair(g.kz, g.kz), kd = pair(g.kd, g.kd), kt = pair(-g.kt, -g.kt);
-    const int end = p.head + r.A;
+    const Inner n = ALIKE ? inner_of<V>(r, p) : Inner{p.v0, p.v1, -1, -1};
+    const int act_v = KIND == kSearch || act_e < 0 ? -1 : act_e / V;
+    // the gradient's words in place of the logits'
+    auto made = [&](W& w, int v) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const f32x2 d = elements_less<T>(w.z, i, M, g.M), pr = ex2_2(fma2(d, L, lp));
+            f32x2 y = fma2(kz, d, k0);
+            if (KIND == kClippedRef) y = fma2(kd, fma2(elements_less<T>(w.x, i, C, g.C), minus, d), y);
+            y = mul2(y, pr);
+            if (KIND == kSearch) y = fma2(kt, elements<float>(w.x, i), y);
+            halves(y, o[2 * i], o[2 * i + 1]);
+        }
+        if (KIND != kSearch && v == act_v)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (act_e % V == i) o[i] += g.ka;
+        if (sizeof(T) == 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w.z[i] = __float_as_uint(o[i % V]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w.z[i] = pack2<T>(o[(2 * i) % V], o[(2 * i + 1) % V]);
+    };
+    auto put = [&](const W& w, int v) {
+        if (ALIKE) *(uint4*)(grad + v * V) = make_uint4(w.z[0], w.z[1], w.z[2], w.z[3]);
+        else w.store_z(p, v);
+    };
+    int v = p.v0 + tid;
+    if (SHORT && ALIKE) {
+        const int end = p.head + r.A;
 #pragma unroll 2
-    for (int v = p.v0 + tid; v < p.v1; v += stride) {
-        uint32_t z[4] = {0, 0, 0, 0}, x[XV / 4];
-        if (live) {
-            float o[V];
-            load16(p.zs + (v - p.v0) * 16, z);
-            if (KIND != kClipped)
-#pragma unroll
-                for (int i = 0; i < XV / 16; ++i) load16(p.xs + (v - p.v0) * XV + 16 * i, x + 4 * i);
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const f32x2 d = add2(elements<T>(z, i), M), pr = ex2_2(fma2(d, L, lp));
-                f32x2 y = fma2(kz, d, k0);
-                if (KIND == kClippedRef) y = fma2(kd, fma2(add2(elements<T>(x, i), C), minus, d), y);
-                y = mul2(y, pr);
-                if (KIND == kSearch) y = fma2(kt, elements<float>(x, i), y);
-                halves(y, o[2 * i], o[2 * i + 1]);
+        for (; v < p.v1; v += stride) {
+            W w;
+            w.z[0] = w.z[1] = w.z[2] = w.z[3] = 0u;
+            if (live) {
+                w.load_z(p, v);
+                w.load_x(p, v);
+                made(w, v);
             }
-            if (KIND != kSearch && (unsigned)act_e - (unsigned)(v * V) < (unsigned)V)
+            if (v != n.first && v != n.last) {
+                put(w, v);
+            } else {
+                const int at = v * V;
+                T* to = grad + at;
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (act_e == v * V + i) o[i] += g.ka;
-            if (sizeof(T) == 4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = __float_as_uint(o[i % V]);
-            else
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = pack2<T>(o[(2 * i) % V], o[(2 * i + 1) % V]);
+                for (int i = 0; i < V; ++i) {
+                    const uint32_t word = w.z[i * (int)sizeof(T) / 4];
+                    if (at + i >= p.head && at + i < end) {
+                        if (sizeof(T) == 4) *(uint32_t*)(to + i) = word;
+                        else *(unsigned short*)(to + i) = (unsigned short)(i & 1 ? word >> 16 : word);
+                    }
+                }
+            }
         }
-        const int e = v * V;
-        if (!ALIKE) {
-            store16(p.zs + (v - p.v0) * 16, z);
-        } else if (e >= p.head && e + V <= end) {
-            *(uint4*)(grad + e) = make_uint4(z[0], z[1], z[2], z[3]);
-        } else {
-            uint8_t* zp = p.zs + (v - p.v0) * 16;
-            store16(zp, z);
-            for (int i = max(p.head - e, 0); i < min(V, end - e); ++i) grad[e + i] = ((const T*)zp)[i];
+        return;
+    }
+    if (v < n.lo) v += stride;
+    if (live) {
+        for (; v + (U - 1) * stride < n.hi; v += U * stride) {
+            W w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) { w[u].load_z(p, v + u * stride); w[u].load_x(p, v + u * stride); }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                made(w[u], v + u * stride);
+                put(w[u], v + u * stride);
+            }
         }
+        for (; v < n.hi; v += stride) {
+            W w;
+            w.load_z(p, v);
+            w.load_x(p, v);
+            made(w, v);
+            put(w, v);
+        }
+    } else {
+        W w;
+        w.z[0] = w.z[1] = w.z[2] = w.z[3] = 0u;
+        for (; v < n.hi; v += stride) put(w, v);
+    }
+    if (!ALIKE) return;
+    for (int k = 0; k < 2; ++k) {
+        const int e = k ? n.last : n.first;
+        if (e < 0 || (k ? v != e : tid != 0)) continue;
+        W w;
+        w.z[0] = w.z[1] = w.z[2] = w.z[3] = 0u;
+        if (live) {
+            w.load_z(p, e);
+            w.load_x(p, e);
+            made(w, e);
+        }
+        w.store_z(p, e);
+        const int at = e * V;
+        for (int i = max(p.head - at, 0); i < min(V, p.head + r.A - at); ++i) grad[at + i] = ((const T*)p.zs)[(e - p.v0) * V + i];
     }
 }
 
@@ -551,56 +762,54 @@ __device__ __forceinline__ void copy_vectors(const PolicyRows& r, long long row,
 }
 
 // ---- short rows --------------------------------------------------------------------
-// LANES lanes a row, 32 / LANES adjacent rows a warp; each warp has slots of its own and fills them itself.
+// LANES lanes a row, 32 / LANES adjacent rows a warp; each warp has slots of its own and fills them itself.  While a warp waits
+// for its copies the SM's others work: with two slots a warp, and so half the warps, 65,536 x 362 took 90 us, with one 52.
 template <typename T, int KIND, int LANES, bool ALIKE>
-__global__ void __launch_bounds__(128, 6)
+__global__ void __launch_bounds__(128, LANES == 32 ? 4 : 6)
 policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {
-    constexpr int R = 32 / LANES;
+    constexpr int R = 32 / LANES, U = LANES == 32 ? 4 : 2;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int abort_flag;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, tid = lane % LANES, mine_of = lane / LANES;
-    const int warp_bytes = sh.slots * (R * sh.slot_bytes + 16);
+    const int warp_bytes = R * sh.slot_bytes + 16;
     uint8_t* const mine = smem + warp * warp_bytes;
-    const uint32_t mine_s = ptx::smem_u32(mine), bars = mine_s + sh.slots * R * sh.slot_bytes;
-    if (ALIKE && lane == 0)
-        for (int s = 0; s < sh.slots; ++s) ptx::mbar_init(bars + 16 * s, R + (r.bits ? 32 : 0));
+    const uint32_t mine_s = ptx::smem_u32(mine), full = mine_s + R * sh.slot_bytes;
+    if (ALIKE && lane == 0) ptx::mbar_init(full, R + (r.bits ? 32 : 0));
     if (threadIdx.x == 0) abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
 
     const long long first = ((long long)blockIdx.x * warps + warp) * R + mine_of, step = (long long)gridDim.x * warps * R;
-    // This team's row into slot s; rows beyond the last are announced too, so that the warp's barrier completes.
-    auto fill = [&](long long row, int s, float4 scalars) {
-        const int at = (s * R + mine_of) * sh.slot_bytes;
-        const uint32_t bar = bars + 16 * s;
+    uint8_t* const at = mine + mine_of * sh.slot_bytes;
+    const uint32_t at_s = mine_s + mine_of * sh.slot_bytes;
+    // This team's row into its slot; rows beyond the last are announced too, so that the warp's barrier completes.
+    auto fill = [&](long long row, float4 scalars) {
         const bool is = row < r.n;
         if (r.bits) {
             if (is)
-                for (int i = tid; i < (r.A + 31) / 32; i += LANES) copy_word_async(mine_s + at + sh.mask_at + 4 * i, r.bits + row * r.mask_words + i);
-            arrive_after_copies(bar);
+                for (int i = tid; i < (r.A + 31) / 32; i += LANES) copy_word_async(at_s + sh.mask_at + 4 * i, r.bits + row * r.mask_words + i);
+            arrive_after_copies(full);
         }
         if (tid == 0) {
-            *(float4*)(mine + at) = scalars;
+            *(float4*)at = scalars;
             const Place p = place_of<T, KIND, ALIKE>(r, is ? row : 0);
-            copy_vectors<T, KIND>(r, row, p, 0, p.vecs, mine_s + at, sh.x_at, bar, is && scalars.x != 0.f);
+            copy_vectors<T, KIND>(r, row, p, 0, p.vecs, at_s, sh.x_at, full, is && scalars.x != 0.f);
         }
     };
-    float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);          // scalars of the next row to be copied
+    float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);          // scalars of the row after the one in the slot
     if (ALIKE) {
-        for (int s = 0; s < sh.slots; ++s)
-            if (first - mine_of + s * step < r.n) fill(first + s * step, s, scalars_of(r, KIND, first + s * step));
-        if (tid == 0) ahead = scalars_of(r, KIND, first + sh.slots * step);
+        if (first - mine_of < r.n) fill(first, scalars_of(r, KIND, first));
+        if (tid == 0) ahead = scalars_of(r, KIND, first + step);
     }
-    int slot = 0;
     uint32_t parity = 0;
     for (long long row = first; row - mine_of < r.n; row += step) {        // the same turns for the whole warp
         const bool is = row < r.n;
-        uint8_t* const at = mine + (slot * R + mine_of) * sh.slot_bytes;
         const Place pl = place_of<T, KIND, ALIKE>(r, is ? row : 0);
         const Part p{at + kHeader, at + sh.x_at, (const uint32_t*)(at + sh.mask_at), 0, pl.head, pl.vecs, 0, is ? pl.vecs : 0, pl.first_out, pl.last_out};
         float4 scalars;
         if (ALIKE) {
-            if (!ptx::mbar_wait_warp(bars + 16 * slot, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+            if (!ptx::mbar_wait_warp(full, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+            parity ^= 1;
             scalars = *(const float4*)at;
         } else {
             scalars = scalars_of(r, KIND, row);
@@ -612,7 +821,10 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;       // the action's element of the row
         bool live = is && w != 0.f, apart = false;
         uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
-        if (live) pass_max<T, KIND, ALIKE>(r, row, p, tid, LANES, &top_z, &top_x);
+        const bool some = live && pass_max<T, KIND, ALIKE, U, (LANES < 32)>(r, row, p, tid, LANES, &top_z, &top_x);
+        // rows without a legal action are left out
+        if (LANES == 32) live = __any_sync(~0u, some);
+        else live = (__ballot_sync(~0u, some) >> (lane & ~(LANES - 1))) & ((1u << (LANES & 31)) - 1);
         Sums q;
         q.m = team_max_nan<LANES>(word_top<T>(top_z));
         q.c = KIND == kClippedRef ? team_max_nan<LANES>(word_top<T>(top_x)) : 0.f;
@@ -624,7 +836,7 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
             careful_row<T, KIND>(r, __shfl_sync(~0u, row, __ffs(m) - 1));
         live = live && !apart;
         q.s = q.t = q.a = q.b = 0.f;
-        if (live) pass_sums<T, KIND>(p, tid, LANES, q);
+        if (live) pass_sums<T, KIND, U>(p, tid, LANES, q);
         q.s = team_sum<LANES>(q.s);
         q.t = team_sum<LANES>(q.t);
         if (KIND != kClipped) { q.a = team_sum<LANES>(q.a); q.b = team_sum<LANES>(q.b); }
@@ -633,25 +845,24 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && live;
         if (tid == 0 && is && !apart) put_out(r, row, live, out);
         T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
-        if (!apart) pass_grad<T, KIND, ALIKE>(r, p, tid, LANES, live, g, act_e, grad);
+        if (!apart) pass_grad<T, KIND, ALIKE, U, (LANES < 32)>(r, p, tid, LANES, live, g, act_e, grad);
         if (ALIKE) {
             // the slot's next copy comes behind what was read and written here
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (row - mine_of + sh.slots * step < r.n) {
-                fill(row + sh.slots * step, slot, ahead);
-                if (tid == 0) ahead = scalars_of(r, KIND, row + (sh.slots + 1) * step);
+            if (row - mine_of + step < r.n) {
+                fill(row + step, ahead);
+                if (tid == 0) ahead = scalars_of(r, KIND, row + 2 * step);
             }
         } else {
             __syncwarp();
             if (!apart) copy_out<T>(r, p, tid, LANES, grad);
             __syncwarp();
         }
-        if (++slot == sh.slots) { slot = 0; parity ^= 1; }
     }
     if (ALIKE && abort_flag) {                   // a wait ran out: what is still in flight is waited for once more, within the same limit
         int none = 0;
-        for (int s = 0; s < sh.slots; ++s) ptx::mbar_wait(bars + 16 * s, s >= slot ? parity : parity ^ 1, &none);
+        ptx::mbar_wait(full, parity ^ 1, &none);
     }
 }
 
@@ -659,25 +870,11 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ void named_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-// Bounded wait on a barrier that the cluster's other CTAs arrive at.
-__device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    for (uint32_t i = 0; i < ptx::kSpinLimit; ++i) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
-        if ((i & 255) == 255 && *abort_flag) return false;
-    }
-    return false;
-}
-
 // What a warp or a CTA found of a row, relative to its own largest logit m and reference logit c - or to 0 where it has no
 // ordinary one: its terms are 0 then.
 template <typename T>
 __device__ __forceinline__ float base_of(float top) { return top < Lowest<T>::kValue / 2 ? 0.f : top; }
-// Entries (m, c, s, t | a, b, za, -), one a lane, none in lanes from n on, as one.
+// Entries (m, c, s, t | a, b, za, whether any action is legal), one a lane, none in lanes from n on, as one.
 template <typename T, int KIND>
 __device__ __forceinline__ Sums join_entries(const float (*entry)[8], int n) {
     const int lane = threadIdx.x % 32;
@@ -699,37 +896,29 @@ __device__ __forceinline__ Sums join_entries(const float (*entry)[8], int n) {
             q.b = hi.y == 0.f ? 0.f : hi.y * ex2(dc * kLog2e);
         }
     }
-    q.s = team_sum(q.s); q.t = team_sum(q.t);
-    if (KIND != kClipped) { q.a = team_sum(q.a); q.b = team_sum(q.b); }
+    const float sum = four_sums(q.s, q.t, q.a, q.b);
+    q.s = __shfl_sync(~0u, sum, 0); q.t = __shfl_sync(~0u, sum, 1); q.a = __shfl_sync(~0u, sum, 2); q.b = __shfl_sync(~0u, sum, 3);
     return q;
 }
 
-// Three kinds of warps that meet at barriers in shared memory only: the workers, which go over a row's vectors - the sums
-// of a row, then the gradient of the row before, whose sums have been joined meanwhile; one that joins the workers' sums
-// and the cluster's; one that copies rows ahead.
+// A CTA, or a cluster's CTAs, a row.  A warp's sums are relative to its own maxima and are joined by every warp at once, so
+// that a row costs one meeting of its warps, and one more before its slot takes the next row; while a CTA waits for its
+// copy the SM's others work.
 template <typename T, int KIND, bool ALIKE>
-__global__ void __launch_bounds__(512, 2)
+__global__ void __launch_bounds__(256, 3)
 policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), U = 2;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(16) float part[2][16][8];        // the workers' sums, by turns
-    __shared__ __align__(16) float joined[2][8][8];       // the cluster's CTAs' sums, by turns
-    __shared__ __align__(16) float found[2][12];          // what comes of a row: RowGrad; live; apart
-    __shared__ __align__(8) unsigned long long full_bar[4], empty_bar[4], sums_bar[2], found_bar[2], join_bar;
+    __shared__ __align__(16) float part[2][32][8];        // the sums of the cluster's warps, by turns
+    __shared__ __align__(8) unsigned long long full_bar;
     __shared__ int abort_flag;
     uint32_t cta, ctas;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32 - 2, threads = 32 * warps;
-    const uint32_t smem_s = ptx::smem_u32(smem), full = ptx::smem_u32(full_bar), empty = ptx::smem_u32(empty_bar);
-    const uint32_t sums = ptx::smem_u32(sums_bar), ready = ptx::smem_u32(found_bar), join = ptx::smem_u32(&join_bar);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, threads = blockDim.x, warps = threads / 32;
+    const uint32_t smem_s = ptx::smem_u32(smem), full = ptx::smem_u32(&full_bar);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < sh.slots; ++s) {
-            ptx::mbar_init(full + 8 * s, 1 + (ALIKE && r.bits ? 32 : 0));
-            ptx::mbar_init(empty + 8 * s, warps + 1);
-        }
-        for (int i = 0; i < 2; ++i) { ptx::mbar_init(sums + 8 * i, warps); ptx::mbar_init(ready + 8 * i, 1); }
-        ptx::mbar_init(join, ctas);
+        ptx::mbar_init(full, 1 + (r.bits ? 32 : 0));
         abort_flag = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -738,181 +927,120 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
     if (ctas > 1) cluster_barrier();
     const int v0 = (int)cta * sh.seg;
     const long long first = blockIdx.x / ctas, step = gridDim.x / ctas;
-    // A wait that runs out is noted; the loops go on without waiting, so that every warp comes to its end.
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (!ptx::mbar_wait_warp(bar, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
-    };
-    auto part_of = [&](int slot) {
-        uint8_t* const at = smem + slot * sh.slot_bytes;
-        const int4 h = *(const int4*)(at + 16);
-        return Part{at + kHeader, at + sh.x_at, (const uint32_t*)(at + sh.mask_at), max(v0 * V - h.x, 0) >> 5, h.x, h.y,
-                    v0, min(h.y, v0 + sh.seg), (h.w & 1) != 0, (h.w & 2) != 0};
-    };
-    auto put_header = [&](int slot, float4 scalars, const Place& p) {
-        uint8_t* const at = smem + slot * sh.slot_bytes;
-        *(float4*)at = scalars;
-        *(int4*)(at + 16) = make_int4(p.head, p.vecs, 0, (p.first_out ? 1 : 0) | (p.last_out ? 2 : 0));
-    };
-    int slot = 0, turn = 0;                      // turn counts the rows that are not left out for their weight
-    uint32_t parity = 0;
-
-    if (warp == warps + 1) {
-        if (ALIKE) {
-            float4 ahead = scalars_of(r, KIND, first);
-            for (long long row = first; row < r.n; row += step) {
-                const float4 scalars = ahead;
-                ahead = scalars_of(r, KIND, row + step);
-                if (row >= first + sh.slots * step) wait(empty + 8 * slot, parity ^ 1);
-                const uint32_t at_s = smem_s + slot * sh.slot_bytes, bar = full + 8 * slot;
-                const Place p = place_of<T, KIND, ALIKE>(r, row);
-                const int v1 = min(p.vecs, v0 + sh.seg);
-                if (r.bits) {
-                    const int w0 = max(v0 * V - p.head, 0) >> 5, w1 = (min(v1 * V - p.head, r.A) - 1) >> 5;
-                    for (int i = w0 + lane; i <= w1; i += 32) copy_word_async(at_s + sh.mask_at + 4 * (i - w0), r.bits + row * r.mask_words + i);
-                    arrive_after_copies(bar);
-                }
-                if (lane == 0) {
-                    put_header(slot, scalars, p);
-                    copy_vectors<T, KIND>(r, row, p, v0, v1, at_s, sh.x_at, bar, scalars.x != 0.f);
-                }
-                __syncwarp();
-                if (++slot == sh.slots) { slot = 0; parity ^= 1; }
-            }
-            if (abort_flag) {                    // what is still in flight is waited for once more, within the same limit
-                int none = 0;
-                for (int s = 0; s < sh.slots; ++s) ptx::mbar_wait(full + 8 * s, s >= slot ? parity ^ 1 : parity, &none);
-            }
+    // A row into the slot, by the first warp.
+    auto fill = [&](long long row, float4 scalars) {
+        const Place p = place_of<T, KIND, ALIKE>(r, row);
+        const int v1 = min(p.vecs, v0 + sh.seg);
+        if (r.bits) {
+            const int w0 = max(v0 * V - p.head, 0) >> 5, w1 = (min(v1 * V - p.head, r.A) - 1) >> 5;
+            for (int i = w0 + lane; i <= w1; i += 32) copy_word_async(smem_s + sh.mask_at + 4 * (i - w0), r.bits + row * r.mask_words + i);
+            arrive_after_copies(full);
         }
-    } else if (warp == warps) {
-        for (long long row = first; row < r.n; row += step) {
-            wait(full + 8 * slot, parity);
-            const float4 scalars = *(const float4*)(smem + slot * sh.slot_bytes);
-            if (scalars.x == 0.f) {
-                if (lane == 0 && cta == 0) put_out(r, row, false, RowOut());
-            } else {
-                const int by = turn & 1;
-                wait(sums + 8 * by, (turn >> 1) & 1);
-                Sums q = join_entries<T, KIND>(part[by], warps);
-                q.za = -kInf;
-                if (KIND != kSearch) {
-                    const Part p = part_of(slot);
-                    const int act = __float_as_int(scalars.w), e = act + p.head;
-                    if ((unsigned)act < (unsigned)r.A && e / V >= v0 && e / V < p.v1 &&
-                        (!r.bits || (p.ms[(act >> 5) - p.mask_first] >> (act & 31)) & 1u))
-                        q.za = to_f32(((const T*)p.zs)[e - v0 * V]);
-                }
-                if (ctas > 1) {
-                    // its sums to every CTA of the cluster
-                    if (lane < (int)ctas) {
-                        uint32_t there, bar;
-                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(ptx::smem_u32(joined[by][cta])), "r"(lane));
-                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(join), "r"(lane));
-                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(q.m), "f"(q.c), "f"(q.s), "f"(q.t) : "memory");
-                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + 16), "f"(q.a), "f"(q.b), "f"(q.za), "f"(0.f) : "memory");
-                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-                    }
-                    if (!__all_sync(~0u, cluster_wait(join, turn & 1, &abort_flag))) { abort_flag = 1; atomicExch(sh.error, 4); }
-                    q = join_entries<T, KIND>(joined[by], (int)ctas);
-                }
-                const bool apart = q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2);
-                RowGrad g;
-                RowOut out;
-                const bool live = row_result<KIND>(r, q, scalars.x, scalars.y, scalars.z, &g, &out);
-                if (lane == 0) {
-                    *(float4*)found[by] = make_float4(g.M, g.C, g.lp, g.k0);
-                    *(float4*)(found[by] + 4) = make_float4(g.kz, g.kd, g.ka, g.kt);
-                    found[by][8] = live ? 1.f : 0.f;
-                    found[by][9] = apart ? 1.f : 0.f;
-                    ptx::mbar_arrive(ready + 8 * by);
-                    if (cta == 0 && !apart) put_out(r, row, live, out);
-                }
-                __syncwarp();
-                if (apart && cta == 0) careful_row<T, KIND>(r, row);
-                ++turn;
-            }
-            if (lane == 0) ptx::mbar_arrive(empty + 8 * slot);
-            if (++slot == sh.slots) { slot = 0; parity ^= 1; }
+        if (lane == 0) {
+            *(float4*)smem = scalars;
+            *(int4*)(smem + 16) = make_int4(p.head, p.vecs, 0, (p.first_out ? 1 : 0) | (p.last_out ? 2 : 0));
+            copy_vectors<T, KIND>(r, row, p, v0, v1, smem_s, sh.x_at, full, scalars.x != 0.f);
         }
-    } else {
-        // The gradient of a row whose sums are on their way.
-        auto finish = [&](long long row, int s, int by) {          // by: its turn, -1 when it is left out for its weight
-            const Part p = part_of(s);
-            RowGrad g;
-            bool live = false, apart = false;
-            int act_e = -1;
-            if (by >= 0) {
-                wait(ready + 8 * (by & 1), (by >> 1) & 1);
-                const float* f = found[by & 1];
-                const float4 lo = *(const float4*)f, hi = *(const float4*)(f + 4);
-                g = RowGrad{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                live = f[8] != 0.f;
-                apart = f[9] != 0.f;
-                if (KIND != kSearch) {
-                    const int act = __float_as_int(((const float*)(smem + s * sh.slot_bytes))[3]);
-                    if ((unsigned)act < (unsigned)r.A) act_e = act + p.head;
-                }
-            }
-            T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
-            if (!apart) pass_grad<T, KIND, ALIKE>(r, p, threadIdx.x, threads, live, g, act_e, grad);
-            if (ALIKE) {
-                // the slot's next copy comes behind what was read and written here
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(empty + 8 * s);
-            } else {
-                named_sync(1, threads);
-                if (!apart) copy_out<T>(r, p, threadIdx.x, threads, grad);
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(empty + 8 * s);
-            }
-        };
-        int before = -1, before_turn = -1;       // slot and turn of the row that is to be finished
-        for (long long row = first; row < r.n; row += step) {
-            if (!ALIKE) {
-                const float4 scalars = scalars_of(r, KIND, row);
-                const Place pl = place_of<T, KIND, ALIKE>(r, row);
-                if (row >= first + sh.slots * step) wait(empty + 8 * slot, parity ^ 1);
-                if (threadIdx.x == 0) put_header(slot, scalars, pl);
-                named_sync(1, threads);
-                if (scalars.x != 0.f) copy_in<T, KIND>(r, row, part_of(slot), threadIdx.x, threads);
-                named_sync(1, threads);
-                if (threadIdx.x == 0) ptx::mbar_arrive(full + 8 * slot);
-            }
-            wait(full + 8 * slot, parity);
-            const bool live = *(const float*)(smem + slot * sh.slot_bytes) != 0.f;
-            if (live) {
-                const Part p = part_of(slot);
-                uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
-                pass_max<T, KIND, ALIKE>(r, row, p, threadIdx.x, threads, &top_z, &top_x);
-                const float top = warp_max_nan(word_top<T>(top_z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
-                Sums q;
-                q.m = base_of<T>(top);
-                q.c = KIND == kClippedRef ? base_of<T>(top_ref) : 0.f;
-                pass_sums<T, KIND>(p, threadIdx.x, threads, q);
-                q.s = team_sum(q.s);
-                q.t = team_sum(q.t);
-                if (KIND != kClipped) { q.a = team_sum(q.a); q.b = team_sum(q.b); }
-                if (lane == 0) {
-                    float* to = part[turn & 1][warp];
-                    *(float4*)to = make_float4(top, top_ref, q.s, q.t);
-                    *(float4*)(to + 4) = make_float4(q.a, q.b, 0.f, 0.f);
-                }
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(sums + 8 * (turn & 1));
-            }
-            if (before >= 0) finish(row - step, before, before_turn);
-            before = slot;
-            before_turn = live ? turn++ : -1;
-            if (++slot == sh.slots) { slot = 0; parity ^= 1; }
-        }
-        if (before >= 0) finish(first + (r.n - 1 - first) / step * step, before, before_turn);
+    };
+    float4 ahead;                                // scalars of the row after the one in the slot
+    if (ALIKE && warp == 0) {
+        if (first < r.n) fill(first, scalars_of(r, KIND, first));
+        ahead = scalars_of(r, KIND, first + step);
     }
-    __syncwarp();
+    uint32_t parity = 0;
+    int turn = 0;
+    for (long long row = first; row < r.n; row += step) {
+        float4 scalars;
+        Place pl;
+        if (ALIKE) {
+            if (!ptx::mbar_wait_warp(full, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+            parity ^= 1;
+            scalars = *(const float4*)smem;
+            const int4 h = *(const int4*)(smem + 16);
+            pl = Place{h.x, h.y, (h.w & 1) != 0, (h.w & 2) != 0};
+        } else {
+            scalars = scalars_of(r, KIND, row);
+            pl = place_of<T, KIND, ALIKE>(r, row);
+        }
+        const Part p{smem + kHeader, smem + sh.x_at, (const uint32_t*)(smem + sh.mask_at), max(v0 * V - pl.head, 0) >> 5, pl.head, pl.vecs,
+                     v0, min(pl.vecs, v0 + sh.seg), pl.first_out, pl.last_out};
+        const float w = scalars.x;
+        if (!ALIKE) {
+            if (w != 0.f) copy_in<T, KIND>(r, row, p, threadIdx.x, threads);
+            __syncthreads();
+        }
+        const int act = KIND == kSearch ? -1 : __float_as_int(scalars.w);
+        const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;       // the action's element of the row
+        bool live = w != 0.f, apart = false;
+        RowGrad g;
+        RowOut out;
+        if (live) {                              // the same in the whole team
+            uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
+            const bool some = __any_sync(~0u, pass_max<T, KIND, ALIKE, U, false>(r, row, p, threadIdx.x, threads, &top_z, &top_x));
+            const float top = warp_max_nan(word_top<T>(top_z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
+            __syncwarp();
+            // the action's logit: of a cluster, by the warp that has its vector
+            const int act_at = KIND != kSearch && act_e >= v0 * V && act_e < p.v1 * V && (!r.bits || (p.ms[(act >> 5) - p.mask_first] >> (act & 31)) & 1u)
+                                   ? act_e - v0 * V : -1;
+            float za = -kInf;
+            if (KIND != kSearch && ctas > 1 && act_at >= 0 && act_at / V % threads / 32 == warp) za = to_f32(((const T*)p.zs)[act_at]);
+            Sums q;
+            q.m = base_of<T>(top);
+            q.c = KIND == kClippedRef ? base_of<T>(top_ref) : 0.f;
+            pass_sums<T, KIND, U>(p, threadIdx.x, threads, q);
+            const float sum = four_sums(q.s, q.t, q.a, q.b);
+            float (*all)[8] = part[turn];
+            turn ^= 1;
+            float* const mine = all[cta * warps + warp];
+            if (ctas == 1) {
+                if (lane < 4) mine[2 + lane] = sum;
+                else if (lane == 4) { mine[0] = top; mine[1] = top_ref; mine[6] = -kInf; mine[7] = some ? 1.f : 0.f; }
+                __syncthreads();
+            } else {
+                const float s = __shfl_sync(~0u, sum, 0), t = __shfl_sync(~0u, sum, 1), a = __shfl_sync(~0u, sum, 2), b = __shfl_sync(~0u, sum, 3);
+                if (lane < (int)ctas) {
+                    uint32_t there;
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(ptx::smem_u32(mine)), "r"(lane));
+                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(top), "f"(top_ref), "f"(s), "f"(t) : "memory");
+                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + 16), "f"(a), "f"(b), "f"(za), "f"(some ? 1.f : 0.f) : "memory");
+                }
+                cluster_barrier();
+            }
+            q = join_entries<T, KIND>(all, (int)ctas * warps);
+            if (KIND != kSearch && ctas == 1 && act_at >= 0) q.za = to_f32(((const T*)p.zs)[act_at]);
+            const bool legal_one = __any_sync(~0u, lane < (int)ctas * warps && all[lane][7] != 0.f);      // else the row is left out
+            apart = legal_one && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2));
+            live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && legal_one;
+            if (apart && warp == 0 && cta == 0) careful_row<T, KIND>(r, row);
+        }
+        if (threadIdx.x == 0 && cta == 0 && !apart) put_out(r, row, live, out);
+        T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
+        if (!apart) pass_grad<T, KIND, ALIKE, U, false>(r, p, threadIdx.x, threads, live, g, act_e, grad);
+        if (ALIKE) {
+            // the next copy comes behind what was read and written here
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncthreads();
+            if (warp == 0 && row + step < r.n) {
+                fill(row + step, ahead);
+                ahead = scalars_of(r, KIND, row + 2 * step);
+            }
+        } else {
+            __syncthreads();
+            if (!apart) copy_out<T>(r, p, threadIdx.x, threads, grad);
+            __syncthreads();
+        }
+    }
+    if (ALIKE && abort_flag && threadIdx.x == 0) {       // a wait ran out: what is still in flight is waited for once more, within the same limit
+        int none = 0;
+        ptx::mbar_wait(full, parity ^ 1, &none);
+    }
+    __syncthreads();
     // and none may leave while another may still write
     if (ctas > 1) cluster_barrier();
 }
 
 // ---- host ---------------------------------------------------------------------------
+constexpr int kSms = 148;
 constexpr int kMostShared = 208 * 1024;          // of a CTA; 227 KB less the kernels' own
 
 // Registers of a thread | SMs << 16, looked up once for each kernel; every device is of the same kind.
@@ -945,7 +1073,7 @@ int launch_warp_rows(const PolicyRows& r, const RowShape& sh, cudaStream_t st) {
     auto kernel = policy_warp_rows_kernel<T, KIND, LANES, ALIKE>;
     int facts;
     if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
-    const int warp_bytes = sh.slots * (R * sh.slot_bytes + 16), fit = 104 * 1024 / warp_bytes, warps = fit < 1 ? 1 : fit > 4 ? 4 : fit;
+    const int warp_bytes = R * sh.slot_bytes + 16, fit = 104 * 1024 / warp_bytes, warps = fit < 1 ? 1 : fit > 4 ? 4 : fit;
     const long long teams = ((long long)r.n + R * warps - 1) / (R * warps), room = resident_ctas(facts, 32 * warps, warps * warp_bytes);
     kernel<<<(unsigned)(teams < room ? teams : room), 32 * warps, warps * warp_bytes, st>>>(r, sh);
     OB200_LAUNCHED("policy_warp_rows_kernel");
@@ -958,15 +1086,32 @@ int launch_cta_rows(const PolicyRows& r, const RowShape& sh, int warps, int ctas
     auto kernel = policy_cta_rows_kernel<T, KIND, ALIKE>;
     int facts;
     if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
-    const int threads = 32 * (warps + 2), smem = sh.slots * sh.slot_bytes;
-    const long long room = resident_ctas(facts, threads, smem) / ctas;
+    const int threads = 32 * warps, smem = sh.slot_bytes;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((r.n < room ? r.n : room) * ctas));
+    cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cfg.attrs = attr; cfg.numAttrs = ctas > 1 ? 1 : 0;
+    long long room = resident_ctas(facts, threads, smem);
+    if (ctas > 1) {
+        // Fewer clusters fit than their CTAs would: not every group of SMs divides into them.  Each cluster has its share of
+        // the rows, so one that had to wait for another's end would double the time.  The answer is kept for the next call
+        // with the same shape.
+        static std::atomic<uint64_t> last[4];
+        std::atomic<uint64_t>& slot = last[ctas == 2 ? 0 : ctas == 4 ? 1 : 2];
+        const uint64_t key = (uint64_t)smem << 32 | (uint64_t)threads << 16;
+        uint64_t got = slot.load(std::memory_order_relaxed);
+        if ((got & ~0xFFFFULL) != key) {
+            int n = 0;
+            OB200_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+            got = key | (uint64_t)(n < 1 ? 1 : n);
+            slot.store(got, std::memory_order_relaxed);
+        }
+        room = (long long)(got & 0xFFFF);
+    }
+    cfg.gridDim = dim3((unsigned)((r.n < room ? r.n : room) * ctas));
     cudaLaunchKernelEx(&cfg, kernel, r, sh);
     OB200_LAUNCHED("policy_cta_rows_kernel");
     return OB200_OK;
@@ -979,7 +1124,7 @@ int launch_shape(const PolicyRows& r, cudaStream_t st) {
     RowShape sh{};
     sh.error = device_error_word();
     if (!sh.error) return set_error(OB200_ERR_CUDA, "policy loss: the device's error word is not available");
-    auto lay = [&](int ctas) {                   // fills sh but for the slots
+    auto lay = [&](int ctas) {
         sh.seg = (vecs + ctas - 1) / ctas;
         sh.x_at = kHeader + sh.seg * 16;
         sh.mask_at = sh.x_at + sh.seg * XV;
@@ -988,19 +1133,25 @@ int launch_shape(const PolicyRows& r, cudaStream_t st) {
     };
     if (r.A <= 1024) {
         lay(1);
-        sh.slots = 1;
-        if (ALIKE && sh.slot_bytes <= 2400 && r.n > 8192) return launch_warp_rows<T, KIND, ALIKE ? 8 : 32, ALIKE>(r, sh, st);
-        if (ALIKE && sh.slot_bytes <= 4800 && r.n > 4096) return launch_warp_rows<T, KIND, ALIKE ? 16 : 32, ALIKE>(r, sh, st);
+        // More rows than the device holds warps for at once: several rows a warp, as far as the shared memory of 24 warps
+        // allows (100,000 x 225 fp32: 60 us with 8 lanes a row, 88 with 16, 133 with 32).  Fewer: a warp each (512 x 225: 5.3
+        // us, 8 lanes 7.2).
+        const bool many = r.n > 24 * kSms;
+        if (ALIKE && many && sh.slot_bytes <= 2400) return launch_warp_rows<T, KIND, ALIKE ? 8 : 32, ALIKE>(r, sh, st);
+        if (ALIKE && many && sh.slot_bytes <= 4800) return launch_warp_rows<T, KIND, ALIKE ? 16 : 32, ALIKE>(r, sh, st);
         return launch_warp_rows<T, KIND, 32, ALIKE>(r, sh, st);
     }
-    if ((long long)vecs * (16 + XV) <= 8LL * kMostShared / 2) {
+    if ((long long)vecs * (16 + XV) <= 8LL * kMostShared) {
+        // A row's part takes up to a third of an SM's shared memory (4,096 x 32,768 bf16: 193 us in parts of 65 KB, 232 in
+        // parts of 33 KB).  While SMs are left over, smaller parts (8 x 32,768: 5.6 us with eight CTAs a row, 8.5 with two).
         int ctas = 1;
-        int most = 36 * 1024;
-        while (ctas < 8 && lay(ctas) > most) ctas *= 2;
-        if (2 * lay(ctas) <= kMostShared) {
-            sh.slots = 3 * sh.slot_bytes <= kMostShared ? 3 : 2;
-            const int warps = (sh.seg + 95) / 96;
-            return launch_cta_rows<T, KIND, ALIKE>(r, sh, warps < 2 ? 2 : warps > 14 ? 14 : warps, ctas, st);
+        while (ctas < 8 && lay(ctas) > 72 * 1024) ctas *= 2;
+        while (ctas < 8 && lay(ctas) > 20 * 1024 && (long long)r.n * ctas < 2 * kSms) ctas *= 2;
+        if (lay(ctas) <= kMostShared) {
+            // 64 actions a lane, as few as there may be while every row has SMs of its own; 32 entries of sums at most
+            const int most = ctas == 8 ? 4 : 8, lanes_of = (long long)r.n * ctas < 2 * kSms ? 16 : 64;
+            const int warps = (sh.seg * V + 32 * lanes_of - 1) / (32 * lanes_of);
+            return launch_cta_rows<T, KIND, ALIKE>(r, sh, warps > most ? most : warps, ctas, st);
         }
     }
     policy_long_rows_kernel<T, KIND><<<(unsigned)r.n, 512, 0, st>>>(r);
