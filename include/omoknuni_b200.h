@@ -749,8 +749,8 @@ typedef struct ob200_train_tensor {
  * max_norm, else 1.  Squares are fp32: a gradient beyond 1.8e19 makes the norm
  * infinite.  Where out[0] is not finite out[1] is NaN, which ob200_launch_adamw
  * takes as "leave this step out".  `workspace`: DEVICE,
- * ob200_grad_norm_workspace_bytes() bytes, 8-byte aligned, contents arbitrary;
- * calls that may overlap need one each. */
+ * ob200_grad_norm_workspace_bytes() bytes, 8-byte aligned, zeroed before the first
+ * call; calls that may overlap need one each. */
 int64_t ob200_grad_norm_workspace_bytes(void);
 int ob200_launch_grad_norm(const ob200_train_tensor* tensors, int32_t n_tensors, int32_t grad_dtype, float max_norm,
                            void* workspace, float* out, ob200_stream stream);

@@ -745,7 +745,7 @@ class GradNorm:
         _require(self.out.dtype == torch.float32 and self.out.device == self.device and tuple(self.out.shape) == (2,)
                  and self.out.is_contiguous(), "GradNorm: out is float32 [2] on the gradients' device")
         self.clip = self.out[1:]
-        self.workspace = torch.empty(int(lib().ob200_grad_norm_workspace_bytes()) // 8, dtype=torch.float64, device=self.device)
+        self.workspace = torch.zeros(int(lib().ob200_grad_norm_workspace_bytes()) // 8, dtype=torch.float64, device=self.device)
         self.table = (TrainTensor * len(self.grads))()
         for e, g in zip(self.table, self.grads):
             e.grad, e.numel = g.data_ptr(), g.numel()

@@ -17,9 +17,11 @@ namespace ob200 {
 namespace {
 
 constexpr int kBlock = 256;              // elements that share the scales of 8-bit states
-// Elements of a CTA of AdamW: eight warps, a block each, or two where the states are codes (what a CTA costs besides its
-// elements is a fifth of the instructions with one).
-template <int BITS> constexpr int kChunk = BITS == 8 ? 4096 : 2048;
+// Threads and elements of a CTA of AdamW: a warp takes a block, or two where the states are codes - what a warp costs besides
+// its elements is a fifth of the instructions with one - and CTAs are small there, so that 28 warps fit an SM (24.5 M fp32
+// weights: 63 us, with CTAs of eight warps 67, 5.5 TB/s).
+template <int BITS> constexpr int kThreads = BITS == 8 ? 128 : 256;
+template <int BITS> constexpr int kChunk = 2048;
 template <typename G> constexpr int kNormChunk = 1024 * (16 / (int)sizeof(G));    // of a CTA's turn of the norm: 64 bytes a thread
 constexpr float kE4m3Max = 448.f, kE4m3Least = 0x1p-9f, kScaleFloor = 0x1p-110f;
 constexpr int kNormCtas = 1184;          // partial sums of the norm: eight CTAs per SM
@@ -111,16 +113,18 @@ __device__ __forceinline__ double cta_sum(double v) {
     return a;
 }
 
-// Squares and a thread's sums over a chunk (16 or 32 elements) in fp32, everything beyond in fp64.
+// Squares and a thread's sums over a chunk (16 or 32 elements) in fp32, everything beyond in fp64.  The CTA that ends last
+// adds up what the others left, in their order, and sets the counter back for the next call; a list that takes several
+// launches is added up by the last of them.
+struct NormEnd { float max_norm; float* out; unsigned* ended; int parts; };      // out null: not the last launch; parts ahead of this launch's
 template <typename G, int N>
 __global__ void __launch_bounds__(256)
-grad_norm_part_kernel(const __grid_constant__ Table<N> t, double* __restrict__ part) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // grad_norm_finish_kernel waits for the whole grid
+grad_norm_kernel(const __grid_constant__ Table<N> t, double* part, const NormEnd end) {
     constexpr int V = 16 / sizeof(G);
     double sum = 0.0;
     int c = (int)((long long)t.chunks * blockIdx.x / gridDim.x);
-    const int end = (int)((long long)t.chunks * (blockIdx.x + 1) / gridDim.x);
-    for (int i = entry_of(t, c); c < end; ++c) {
+    const int behind = (int)((long long)t.chunks * (blockIdx.x + 1) / gridDim.x);
+    for (int i = entry_of(t, c); c < behind; ++c) {
         while (i + 1 < t.count && t.chunk0[i + 1] <= c) ++i;
         const Entry& e = t.e[i];
         const long long at = (long long)(c - t.chunk0[i]) * kNormChunk<G>;
@@ -145,20 +149,23 @@ grad_norm_part_kernel(const __grid_constant__ Table<N> t, double* __restrict__ p
         sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
     }
     sum = cta_sum(sum);
-    if (threadIdx.x == 0) part[blockIdx.x] = sum;
-}
-
-__global__ void __launch_bounds__(256)
-grad_norm_finish_kernel(const double* part, int n, float max_norm, float* out) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) sum += part[i];
+    __shared__ int last;
+    if (threadIdx.x == 0) {
+        part[end.parts + blockIdx.x] = sum;
+        __threadfence();
+        last = end.out && atomicInc(end.ended, gridDim.x - 1) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    sum = 0.0;
+    for (int i = threadIdx.x; i < end.parts + (int)gridDim.x; i += 256) sum += __ldcg(part + i);
     sum = cta_sum(sum);
     if (threadIdx.x) return;
     const double norm = sqrt(sum);
-    out[0] = (float)norm;
+    end.out[0] = (float)norm;
     // an infinite norm gives NaN, not 0: the step is to be left out, not made with zeroed gradients
-    out[1] = !isfinite((float)norm) ? __int_as_float(0x7fc00000) : norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f;
+    end.out[1] = !isfinite((float)norm) ? __int_as_float(0x7fc00000) : norm > (double)end.max_norm ? (float)((double)end.max_norm / norm) : 1.f;
 }
 
 // ---- AdamW ----------------------------------------------------------------------
@@ -203,13 +210,13 @@ __device__ __forceinline__ float rcp(float x) {
 // The moments are fused multiply-adds, beta m + ((1 - beta) g) and beta v + ((1 - beta) (g g)), every other product rounded, so
 // that the codes of 8-bit states are a function of the inputs alone.
 template <typename P, typename G, int BITS, int N>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads<BITS>, BITS == 8 ? 7 : 1)
 adamw_kernel(const __grid_constant__ Table<N> t, const __grid_constant__ Step k) {
-    constexpr int NB = kChunk<BITS> / (8 * kBlock);
+    constexpr int NB = kChunk<BITS> / (kThreads<BITS> / 32 * kBlock);
     const int at_entry = entry_of(t, blockIdx.x);
     const Entry& e = t.e[at_entry];
     const int lane = threadIdx.x % 32;
-    const long long first = ((long long)((int)blockIdx.x - t.chunk0[at_entry]) * 8 + threadIdx.x / 32) * NB;
+    const long long first = ((long long)((int)blockIdx.x - t.chunk0[at_entry]) * (kThreads<BITS> / 32) + threadIdx.x / 32) * NB;
     asm volatile("griddepcontrol.wait;" ::: "memory");       // until here nothing but the parameters was read
     const float gs = k.grad_scale ? *k.grad_scale : 1.f;
     if (!isfinite(gs) || first * kBlock >= e.n) return;
@@ -318,7 +325,11 @@ adamw_kernel(const __grid_constant__ Table<N> t, const __grid_constant__ Step k)
         m_top = warp_max(m_top); r_top = warp_max(r_top);
         if (m_top < kScaleFloor) m_top = kScaleFloor;
         if (r_top < kScaleFloor) r_top = kScaleFloor;
-        const float mi = __fdiv_rn(kE4m3Max, m_top), ri = __fdiv_rn(kE4m3Max, r_top);
+        // four divisions in one, a lane each: 448 / top for the codes, top / 448 for the scales
+        const float one_top = lane & 1 ? r_top : m_top, ratio = __fdiv_rn(lane & 2 ? one_top : kE4m3Max, lane & 2 ? kE4m3Max : one_top);
+        const float mi = __shfl_sync(~0u, ratio, 0), ri = __shfl_sync(~0u, ratio, 1);
+        if (lane == 2) e.ms[first + b] = ratio;
+        if (lane == 3) e.vs[first + b] = ratio;
         const f32x2 mi2 = pair(mi, mi), ri2 = pair(ri, ri);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -352,7 +363,6 @@ adamw_kernel(const __grid_constant__ Table<N> t, const __grid_constant__ Step k)
                 v8[j] = (uint8_t)(vc[b][i / 4] >> (8 * (i % 4)));
             }
         }
-        if (lane == 0) { e.ms[first + b] = __fdiv_rn(m_top, kE4m3Max); e.vs[first + b] = __fdiv_rn(r_top, kE4m3Max); }
     }
 }
 
@@ -394,26 +404,28 @@ int check_list(const char* who, const ob200_train_tensor* t, int n) {
 }
 
 template <typename G, int N>
-int norm_launches(const ob200_train_tensor* tensors, int n, double* part, int* parts, cudaStream_t st) {
+int norm_launches(const ob200_train_tensor* tensors, int n, double* part, float max_norm, float* out, cudaStream_t st) {
     Table<N> t;
-    int next = 0;
+    int next = 0, parts = 0;
     long long chunks;
-    while (fill_table(&t, tensors, n, kNormChunk<G>, Wide{1, 16, 1}, &next, &chunks)) {
-        // each launch its own partial sums; lists of more than one launch share the places out
-        const int room = kNormCtas - *parts, more = (n - next + N - 1) / N;
+    do {
+        fill_table(&t, tensors, n, kNormChunk<G>, Wide{1, 16, 1}, &next, &chunks);
+        // lists of more than one launch share the places of partial sums out
+        const int room = kNormCtas - parts, more = (n - next + N - 1) / N;
         if (room < 1) return set_error(OB200_ERR_TOO_LARGE, "ob200_launch_grad_norm: too many tensors");
-        const int ctas = (int)std::min<long long>(chunks, std::max(1, room / (1 + more)));
-        grad_norm_part_kernel<G, N><<<ctas, 256, 0, st>>>(t, part + *parts);
-        OB200_LAUNCHED("grad_norm_part_kernel");
-        *parts += ctas;
-    }
+        const int ctas = (int)std::max(1LL, std::min<long long>(chunks, std::max(1, room / (1 + more))));
+        const NormEnd end{max_norm, next == n ? out : nullptr, (unsigned*)(part + kNormCtas), parts};
+        grad_norm_kernel<G, N><<<ctas, 256, 0, st>>>(t, part, end);
+        OB200_LAUNCHED("grad_norm_kernel");
+        parts += ctas;
+    } while (next < n);
     return OB200_OK;
 }
 
 template <typename G>
-int norm_typed(const ob200_train_tensor* tensors, int n, double* part, int* parts, cudaStream_t st) {
-    if (n <= kSmallTable) return norm_launches<G, kSmallTable>(tensors, n, part, parts, st);
-    return n <= kMiddleTable ? norm_launches<G, kMiddleTable>(tensors, n, part, parts, st) : norm_launches<G, kLargeTable>(tensors, n, part, parts, st);
+int norm_typed(const ob200_train_tensor* tensors, int n, double* part, float max_norm, float* out, cudaStream_t st) {
+    if (n <= kSmallTable) return norm_launches<G, kSmallTable>(tensors, n, part, max_norm, out, st);
+    return n <= kMiddleTable ? norm_launches<G, kMiddleTable>(tensors, n, part, max_norm, out, st) : norm_launches<G, kLargeTable>(tensors, n, part, max_norm, out, st);
 }
 
 template <typename P, typename G, int BITS, int N>
@@ -422,7 +434,7 @@ int adamw_launches(const ob200_train_tensor* tensors, int n, const Step& k, cuda
     int next = 0;
     long long chunks;
     while (fill_table(&t, tensors, n, kChunk<BITS>, Wide{4 * sizeof(P), 4 * sizeof(G), BITS == 32 ? 16 : 4}, &next, &chunks)) {
-        OB200_CUDA_OK(launch_dependent(adamw_kernel<P, G, BITS, N>, dim3((unsigned)chunks), dim3(256), 0, st, t, k));
+        OB200_CUDA_OK(launch_dependent(adamw_kernel<P, G, BITS, N>, dim3((unsigned)chunks), dim3(kThreads<BITS>), 0, st, t, k));
         OB200_LAUNCHED("adamw_kernel");
     }
     return OB200_OK;
@@ -472,7 +484,7 @@ using namespace ob200;
 
 extern "C" {
 
-int64_t ob200_grad_norm_workspace_bytes(void) { return kNormCtas * (int64_t)sizeof(double); }
+int64_t ob200_grad_norm_workspace_bytes(void) { return (kNormCtas + 1) * (int64_t)sizeof(double); }
 
 int ob200_launch_grad_norm(const ob200_train_tensor* tensors, int32_t n_tensors, int32_t grad_dtype, float max_norm, void* workspace,
                            float* out, ob200_stream stream) {
@@ -489,15 +501,9 @@ int ob200_launch_grad_norm(const ob200_train_tensor* tensors, int32_t n_tensors,
     if (int rc = require_device()) return rc;
     cudaStream_t st = as_stream(stream);
     double* part = (double*)workspace;
-    int parts = 0, rc;
-    if (grad_dtype == OB200_DTYPE_BF16) rc = norm_typed<__nv_bfloat16>(tensors, n_tensors, part, &parts, st);
-    else if (grad_dtype == OB200_DTYPE_F16) rc = norm_typed<__half>(tensors, n_tensors, part, &parts, st);
-    else rc = norm_typed<float>(tensors, n_tensors, part, &parts, st);
-    if (rc) return rc;
-    if (parts) OB200_CUDA_OK(launch_dependent(grad_norm_finish_kernel, dim3(1), dim3(256), 0, st, (const double*)part, parts, max_norm, out));
-    else grad_norm_finish_kernel<<<1, 256, 0, st>>>(part, 0, max_norm, out);
-    OB200_LAUNCHED("grad_norm_finish_kernel");
-    return OB200_OK;
+    if (grad_dtype == OB200_DTYPE_BF16) return norm_typed<__nv_bfloat16>(tensors, n_tensors, part, max_norm, out, st);
+    if (grad_dtype == OB200_DTYPE_F16) return norm_typed<__half>(tensors, n_tensors, part, max_norm, out, st);
+    return norm_typed<float>(tensors, n_tensors, part, max_norm, out, st);
 }
 
 int ob200_launch_adamw(const ob200_train_tensor* tensors, int32_t n_tensors, const ob200_adamw_config* c, ob200_stream stream) {
