@@ -431,17 +431,18 @@ __device__ __forceinline__ Inner inner_of(const PolicyRows& r, const Part& p) {
     return n;
 }
 
-// Bits of the legal actions of vector v; a vector that starts ahead of the row, or ends behind it, has none there.
+// Bits of the legal actions of vector v; the places ahead of the row and behind it have none (the word ahead of the mask's
+// first is 0, what stands behind its last is cut off).
 template <int V>
 __device__ __forceinline__ uint32_t bits_of(const PolicyRows& r, const Part& p, int v) {
     const int j = v * V - p.head;                           // the first element's action; below 0 in the first vector
     uint32_t on = ~0u;
     if (r.bits) {
-        const int i = (j >> 5) - p.mask_first, most = (r.A - 1) >> 5;
-        const uint32_t lo = j < 0 ? 0u : p.ms[i], hi = (j & 31) + V > 32 && (j >> 5) < most ? p.ms[i + 1] : 0u;
-        on = __funnelshift_r(lo, hi, j & 31);
+        const uint32_t* w = p.ms + ((j >> 5) - p.mask_first);
+        on = __funnelshift_r(w[0], w[1], j & 31);
+    } else if (j < 0) {
+        on <<= -j;
     }
-    if (j < 0) on &= ~0u << -j;
     if (j + V > r.A) on &= ~(~0u << (r.A - j));
     return on;
 }
@@ -497,9 +498,9 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
             W w;
             w.load_z(p, v);
             w.load_x(p, v);
-            const int j = v * V - p.head, i = (j >> 5) - p.mask_first;
-            uint32_t on = p.ms[i] >> (j & 31);
-            if ((j & 31) + V > 32) on |= p.ms[i + 1] << (32 - (j & 31));
+            const int j = v * V - p.head;
+            const uint32_t* bits = p.ms + ((j >> 5) - p.mask_first);
+            const uint32_t on = __funnelshift_r(bits[0], bits[1], j & 31);
             any |= on & ((1u << V) - 1);
             w.keep(on);
             if (KIND == kSearch) {
@@ -611,8 +612,10 @@ template <typename T, int KIND, bool ALIKE, int U, bool SHORT>
 __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, int tid, int stride, bool live, const RowGrad& g, int act_e, T* grad) {
     constexpr int V = 16 / sizeof(T);
     using W = Vec<T, KIND>;
-    const f32x2 M = pair(-g.M, -g.M), C = pair(-g.C, -g.C), L = pair(kLog2e, kLog2e), minus = pair(-1.f, -1.f);
-    const f32x2 lp = pair(g.lp, g.lp), k0 = pair(g.k0, g.k0), kz = pair(g.kz, g.kz), kd = pair(g.kd, g.kd), kt = pair(-g.kt, -g.kt);
+    const f32x2 M = pair(-g.M, -g.M), C = pair(-g.C, -g.C), L = pair(kLog2e, kLog2e);
+    // kz d + kd (d - d') as (kz + kd) d - kd d'
+    const float kzd = g.kz + g.kd;
+    const f32x2 lp = pair(g.lp, g.lp), k0 = pair(g.k0, g.k0), kz = pair(kzd, kzd), kd = pair(-g.kd, -g.kd), kt = pair(-g.kt, -g.kt);
     const Inner n = ALIKE ? inner_of<V>(r, p) : Inner{p.v0, p.v1, -1, -1};
     const int act_v = KIND == kSearch || act_e < 0 ? -1 : act_e / V;
     // the gradient's words in place of the logits'
@@ -622,7 +625,7 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
         for (int i = 0; i < V / 2; ++i) {
             const f32x2 d = elements_less<T>(w.z, i, M, g.M), pr = ex2_2(fma2(d, L, lp));
             f32x2 y = fma2(kz, d, k0);
-            if (KIND == kClippedRef) y = fma2(kd, fma2(elements_less<T>(w.x, i, C, g.C), minus, d), y);
+            if (KIND == kClippedRef) y = fma2(kd, elements_less<T>(w.x, i, C, g.C), y);
             y = mul2(y, pr);
             if (KIND == kSearch) y = fma2(kt, elements<float>(w.x, i), y);
             halves(y, o[2 * i], o[2 * i + 1]);
@@ -796,6 +799,8 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
             copy_vectors<T, KIND>(r, row, p, 0, p.vecs, at_s, sh.x_at, full, is && scalars.x != 0.f);
         }
     };
+    if (r.bits && tid == 0) *(uint32_t*)(at + sh.mask_at - 4) = 0u;
+    __syncwarp();
     float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);          // scalars of the row after the one in the slot
     if (ALIKE) {
         if (first - mine_of < r.n) fill(first, scalars_of(r, KIND, first));
@@ -919,6 +924,7 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
     const uint32_t smem_s = ptx::smem_u32(smem), full = ptx::smem_u32(&full_bar);
     if (threadIdx.x == 0) {
         ptx::mbar_init(full, 1 + (r.bits ? 32 : 0));
+        if (r.bits) *(uint32_t*)(smem + sh.mask_at - 4) = 0u;
         abort_flag = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1127,8 +1133,8 @@ int launch_shape(const PolicyRows& r, cudaStream_t st) {
     auto lay = [&](int ctas) {
         sh.seg = (vecs + ctas - 1) / ctas;
         sh.x_at = kHeader + sh.seg * 16;
-        sh.mask_at = sh.x_at + sh.seg * XV;
-        sh.slot_bytes = (sh.mask_at + (r.bits ? (sh.seg * V / 32 + 2) * 4 : 0) + 15) / 16 * 16;
+        sh.mask_at = sh.x_at + sh.seg * XV + (r.bits ? 4 : 0);        // behind a word that is 0; a word more than is copied is read
+        sh.slot_bytes = (sh.mask_at + (r.bits ? (sh.seg * V / 32 + 3) * 4 : 0) + 15) / 16 * 16;
         return sh.slot_bytes;
     };
     if (r.A <= 1024) {
