@@ -178,11 +178,19 @@ __device__ __forceinline__ void word_masks(uint32_t on, uint32_t (&m)[4]) {
         asm("prmt.b32 %0, %1, 0, 0xBBAA;" : "=r"(m[2 * i + 1]) : "r"(signs));
     }
 }
-__device__ __forceinline__ void load16(const uint8_t* p, uint32_t* to) {
-    const uint4 v = *(const uint4*)p;
-    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+// 16 bytes and words of shared memory, by their 32-bit address.
+__device__ __forceinline__ void load16(uint32_t at, uint32_t* to) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(to[0]), "=r"(to[1]), "=r"(to[2]), "=r"(to[3]) : "r"(at));
 }
-__device__ __forceinline__ void store16(uint8_t* p, const uint32_t* v) { *(uint4*)p = make_uint4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store16(uint32_t at, const uint32_t* v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+__device__ __forceinline__ uint32_t load_word(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+template <typename T> __device__ __forceinline__ T* in_shared(uint32_t at) { return (T*)__cvta_shared_to_generic(at); }
 
 // ---- what a row comes to --------------------------------------------------------------
 // Sums of a part of a row, relative to its largest logit m and largest reference logit c.
@@ -356,8 +364,7 @@ __device__ __forceinline__ Place place_of(const PolicyRows& r, long long row) {
 
 // A team's part of a row in its slot.
 struct Part {
-    uint8_t *zs, *xs;
-    const uint32_t* ms;                 // words of the mask from mask_first on
+    uint32_t zs, xs, ms;                // addresses in shared memory; ms: words of the mask from mask_first on
     int mask_first, head, vecs, v0, v1; // this part's vectors are [v0, v1)
     bool first_out, last_out;
 };
@@ -438,8 +445,8 @@ __device__ __forceinline__ uint32_t bits_of(const PolicyRows& r, const Part& p, 
     const int j = v * V - p.head;                           // the first element's action; below 0 in the first vector
     uint32_t on = ~0u;
     if (r.bits) {
-        const uint32_t* w = p.ms + ((j >> 5) - p.mask_first);
-        on = __funnelshift_r(w[0], w[1], j & 31);
+        const uint32_t w = p.ms + 4 * ((j >> 5) - p.mask_first);
+        on = __funnelshift_r(load_word(w), load_word(w + 4), j & 31);
     } else if (j < 0) {
         on <<= -j;
     }
@@ -454,9 +461,9 @@ __device__ __noinline__ void fetch_vector(const PolicyRows& r, long long row, co
     const int j = v * V - p.head, at = (v - p.v0) * V;
     for (int i = 0; i < V; ++i)
         if (j + i >= 0 && j + i < r.A) {
-            ((T*)p.zs)[at + i] = ((const T*)r.z)[row * r.z_pitch + j + i];
-            if (KIND == kSearch) ((uint32_t*)p.xs)[at + i] = ((const uint32_t*)r.x)[row * r.x_pitch + j + i];
-            if (KIND == kClippedRef) ((T*)p.xs)[at + i] = ((const T*)r.x)[row * r.x_pitch + j + i];
+            in_shared<T>(p.zs)[at + i] = ((const T*)r.z)[row * r.z_pitch + j + i];
+            if (KIND == kSearch) in_shared<uint32_t>(p.xs)[at + i] = ((const uint32_t*)r.x)[row * r.x_pitch + j + i];
+            if (KIND == kClippedRef) in_shared<T>(p.xs)[at + i] = ((const T*)r.x)[row * r.x_pitch + j + i];
         }
 }
 
@@ -499,8 +506,8 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
             w.load_z(p, v);
             w.load_x(p, v);
             const int j = v * V - p.head;
-            const uint32_t* bits = p.ms + ((j >> 5) - p.mask_first);
-            const uint32_t on = __funnelshift_r(bits[0], bits[1], j & 31);
+            const uint32_t bits = p.ms + 4 * ((j >> 5) - p.mask_first);
+            const uint32_t on = __funnelshift_r(load_word(bits), load_word(bits + 4), j & 31);
             any |= on & ((1u << V) - 1);
             w.keep(on);
             if (KIND == kSearch) {
@@ -711,7 +718,7 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
         }
         w.store_z(p, e);
         const int at = e * V;
-        for (int i = max(p.head - at, 0); i < min(V, p.head + r.A - at); ++i) grad[at + i] = ((const T*)p.zs)[(e - p.v0) * V + i];
+        for (int i = max(p.head - at, 0); i < min(V, p.head + r.A - at); ++i) grad[at + i] = in_shared<const T>(p.zs)[(e - p.v0) * V + i];
     }
 }
 
@@ -721,18 +728,18 @@ __device__ __forceinline__ void copy_in(const PolicyRows& r, long long row, cons
     constexpr int V = 16 / sizeof(T);
     const int j0 = p.v0 * V, j1 = min(p.v1 * V, r.A);
     for (int j = j0 + tid; j < j1; j += stride) {
-        ((T*)p.zs)[j - j0] = ((const T*)r.z)[row * r.z_pitch + j];
-        if (KIND == kSearch) ((uint32_t*)p.xs)[j - j0] = ((const uint32_t*)r.x)[row * r.x_pitch + j];
-        if (KIND == kClippedRef) ((T*)p.xs)[j - j0] = ((const T*)r.x)[row * r.x_pitch + j];
+        in_shared<T>(p.zs)[j - j0] = ((const T*)r.z)[row * r.z_pitch + j];
+        if (KIND == kSearch) in_shared<uint32_t>(p.xs)[j - j0] = ((const uint32_t*)r.x)[row * r.x_pitch + j];
+        if (KIND == kClippedRef) in_shared<T>(p.xs)[j - j0] = ((const T*)r.x)[row * r.x_pitch + j];
     }
     if (r.bits)
-        for (int i = p.mask_first + tid; i <= (j1 - 1) >> 5; i += stride) ((uint32_t*)p.ms)[i - p.mask_first] = r.bits[row * r.mask_words + i];
+        for (int i = p.mask_first + tid; i <= (j1 - 1) >> 5; i += stride) in_shared<uint32_t>(p.ms)[i - p.mask_first] = r.bits[row * r.mask_words + i];
 }
 template <typename T>
 __device__ __forceinline__ void copy_out(const PolicyRows& r, const Part& p, int tid, int stride, T* grad) {
     constexpr int V = 16 / sizeof(T);
     const int j0 = p.v0 * V, j1 = min(p.v1 * V, r.A);
-    for (int j = j0 + tid; j < j1; j += stride) grad[j] = ((const T*)p.zs)[j - j0];
+    for (int j = j0 + tid; j < j1; j += stride) grad[j] = in_shared<const T>(p.zs)[j - j0];
 }
 
 __device__ __forceinline__ float4 scalars_of(const PolicyRows& r, int kind, long long row) {
@@ -810,7 +817,7 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
     for (long long row = first; row - mine_of < r.n; row += step) {        // the same turns for the whole warp
         const bool is = row < r.n;
         const Place pl = place_of<T, KIND, ALIKE>(r, is ? row : 0);
-        const Part p{at + kHeader, at + sh.x_at, (const uint32_t*)(at + sh.mask_at), 0, pl.head, pl.vecs, 0, is ? pl.vecs : 0, pl.first_out, pl.last_out};
+        const Part p{at_s + kHeader, at_s + sh.x_at, at_s + sh.mask_at, 0, pl.head, pl.vecs, 0, is ? pl.vecs : 0, pl.first_out, pl.last_out};
         float4 scalars;
         if (ALIKE) {
             if (!ptx::mbar_wait_warp(full, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
@@ -835,7 +842,7 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         q.c = KIND == kClippedRef ? team_max_nan<LANES>(word_top<T>(top_x)) : 0.f;
         __syncwarp();
         q.za = -kInf;
-        if (KIND != kSearch && live && act_e >= 0 && (!r.bits || (p.ms[act >> 5] >> (act & 31)) & 1u)) q.za = to_f32(((const T*)p.zs)[act_e]);
+        if (KIND != kSearch && live && act_e >= 0 && (!r.bits || (load_word(p.ms + 4 * (act >> 5)) >> (act & 31)) & 1u)) q.za = to_f32(in_shared<const T>(p.zs)[act_e]);
         if (live && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2))) apart = true;
         for (uint32_t m = __ballot_sync(~0u, apart && tid == 0); m; m &= m - 1)
             careful_row<T, KIND>(r, __shfl_sync(~0u, row, __ffs(m) - 1));
@@ -968,7 +975,7 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             scalars = scalars_of(r, KIND, row);
             pl = place_of<T, KIND, ALIKE>(r, row);
         }
-        const Part p{smem + kHeader, smem + sh.x_at, (const uint32_t*)(smem + sh.mask_at), max(v0 * V - pl.head, 0) >> 5, pl.head, pl.vecs,
+        const Part p{smem_s + kHeader, smem_s + sh.x_at, smem_s + sh.mask_at, max(v0 * V - pl.head, 0) >> 5, pl.head, pl.vecs,
                      v0, min(pl.vecs, v0 + sh.seg), pl.first_out, pl.last_out};
         const float w = scalars.x;
         if (!ALIKE) {
@@ -986,10 +993,10 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             const float top = warp_max_nan(word_top<T>(top_z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
             __syncwarp();
             // the action's logit: of a cluster, by the warp that has its vector
-            const int act_at = KIND != kSearch && act_e >= v0 * V && act_e < p.v1 * V && (!r.bits || (p.ms[(act >> 5) - p.mask_first] >> (act & 31)) & 1u)
+            const int act_at = KIND != kSearch && act_e >= v0 * V && act_e < p.v1 * V && (!r.bits || (load_word(p.ms + 4 * ((act >> 5) - p.mask_first)) >> (act & 31)) & 1u)
                                    ? act_e - v0 * V : -1;
             float za = -kInf;
-            if (KIND != kSearch && ctas > 1 && act_at >= 0 && act_at / V % threads / 32 == warp) za = to_f32(((const T*)p.zs)[act_at]);
+            if (KIND != kSearch && ctas > 1 && act_at >= 0 && act_at / V % threads / 32 == warp) za = to_f32(in_shared<const T>(p.zs)[act_at]);
             Sums q;
             q.m = base_of<T>(top);
             q.c = KIND == kClippedRef ? base_of<T>(top_ref) : 0.f;
@@ -1013,7 +1020,7 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
                 cluster_barrier();
             }
             q = join_entries<T, KIND>(all, (int)ctas * warps);
-            if (KIND != kSearch && ctas == 1 && act_at >= 0) q.za = to_f32(((const T*)p.zs)[act_at]);
+            if (KIND != kSearch && ctas == 1 && act_at >= 0) q.za = to_f32(in_shared<const T>(p.zs)[act_at]);
             const bool legal_one = __any_sync(~0u, lane < (int)ctas * warps && all[lane][7] != 0.f);      // else the row is left out
             apart = legal_one && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2));
             live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && legal_one;
