@@ -624,9 +624,24 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
     const float kzd = g.kz + g.kd;
     const f32x2 lp = pair(g.lp, g.lp), k0 = pair(g.k0, g.k0), kz = pair(kzd, kzd), kd = pair(-g.kd, -g.kd), kt = pair(-g.kt, -g.kt);
     const Inner n = ALIKE ? inner_of<V>(r, p) : Inner{p.v0, p.v1, -1, -1};
-    const int act_v = KIND == kSearch || act_e < 0 ? -1 : act_e / V;
+    // The action's element has a term of its own: its thread makes it apart and stores it over the vector's, so that the
+    // loops ask nothing of it.
+    const int act_at = act_e - p.v0 * V;
+    const bool act_mine = KIND != kSearch && live && act_e >= p.v0 * V && act_e < p.v1 * V && act_at / V % stride == tid;
+    float act_grad = 0.f;
+    if (act_mine) {
+        const float d = to_f32(in_shared<const T>(p.zs)[act_at]) - g.M;
+        float y = fmaf(kzd, d, g.k0);
+        if (KIND == kClippedRef) y = fmaf(-g.kd, to_f32(in_shared<const T>(p.xs)[act_at]) - g.C, y);
+        act_grad = fmaf(y, ex2(fmaf(d, kLog2e, g.lp)), g.ka);
+    }
+    auto put_act = [&] {
+        if (!act_mine) return;
+        if (ALIKE) grad[act_e] = from_f32<T>(act_grad);
+        else in_shared<T>(p.zs)[act_at] = from_f32<T>(act_grad);
+    };
     // the gradient's words in place of the logits'
-    auto made = [&](W& w, int v) {
+    auto made = [&](W& w) {
         float o[V];
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
@@ -637,10 +652,6 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
             if (KIND == kSearch) y = fma2(kt, elements<float>(w.x, i), y);
             halves(y, o[2 * i], o[2 * i + 1]);
         }
-        if (KIND != kSearch && v == act_v)
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (act_e % V == i) o[i] += g.ka;
         if (sizeof(T) == 4)
 #pragma unroll
             for (int i = 0; i < 4; ++i) w.z[i] = __float_as_uint(o[i % V]);
@@ -662,7 +673,7 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
             if (live) {
                 w.load_z(p, v);
                 w.load_x(p, v);
-                made(w, v);
+                made(w);
             }
             if (v != n.first && v != n.last) {
                 put(w, v);
@@ -679,6 +690,7 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
                 }
             }
         }
+        put_act();
         return;
     }
     if (v < n.lo) v += stride;
@@ -689,7 +701,7 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
             for (int u = 0; u < U; ++u) { w[u].load_z(p, v + u * stride); w[u].load_x(p, v + u * stride); }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                made(w[u], v + u * stride);
+                made(w[u]);
                 put(w[u], v + u * stride);
             }
         }
@@ -697,7 +709,7 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
             W w;
             w.load_z(p, v);
             w.load_x(p, v);
-            made(w, v);
+            made(w);
             put(w, v);
         }
     } else {
@@ -705,7 +717,10 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
         w.z[0] = w.z[1] = w.z[2] = w.z[3] = 0u;
         for (; v < n.hi; v += stride) put(w, v);
     }
-    if (!ALIKE) return;
+    if (!ALIKE) {
+        put_act();
+        return;
+    }
     for (int k = 0; k < 2; ++k) {
         const int e = k ? n.last : n.first;
         if (e < 0 || (k ? v != e : tid != 0)) continue;
@@ -714,12 +729,13 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
         if (live) {
             w.load_z(p, e);
             w.load_x(p, e);
-            made(w, e);
+            made(w);
         }
         w.store_z(p, e);
         const int at = e * V;
         for (int i = max(p.head - at, 0); i < min(V, p.head + r.A - at); ++i) grad[at + i] = in_shared<const T>(p.zs)[(e - p.v0) * V + i];
     }
+    put_act();
 }
 
 // Without vectors: what a team holds of a row, element by element, into its slot and back.
