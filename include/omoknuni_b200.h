@@ -692,10 +692,10 @@ typedef struct ob200_policy_rows {
                                    itself (same pitch)                            */
     float* loss;                /* [n], or NULL                                   */
     float* stats;               /* [n][4], 16-byte aligned, or NULL               */
-    int64_t logits_pitch;       /* elements between rows, >= n_actions            */
+    int64_t logits_pitch;       /* elements between rows, n_actions to 2^31       */
     int64_t grad_pitch;
     int32_t n;                  /* rows; 0 is a call without work                 */
-    int32_t n_actions;
+    int32_t n_actions;          /* 1 to 2^30                                      */
     int32_t mask_words;         /* >= ceil(n_actions / 32)                        */
     int32_t dtype;              /* OB200_DTYPE_*                                  */
 } ob200_policy_rows;

@@ -813,7 +813,7 @@ class AdamW:
     def step(self, lr, step=None, grad_scale=None):
         """One step.  lr: a number, or a float32 scalar on the device; step: 1 for the first one (default: counted here), or an
         int32 scalar on the device - for captured graphs; grad_scale: a float32 scalar on the device that multiplies every
-        gradient (GradNorm.clip), and leaves the step out when it is not finite."""
+        gradient (GradNorm.clip); when it is not finite weights and states stay as they are, while the count goes on."""
         import torch
         c = self.cfg
         c.grad_scale = None if grad_scale is None else self._scalar(grad_scale, "grad_scale", torch.float32)

@@ -20,17 +20,21 @@ bool rows_meet(const void* a, long long pa, int ea, const void* b, long long pb,
     return off < A * ea || off + A * eb > step;
 }
 
+// Pitches are at most 2^31, so that no offset of n rows leaves 64 bits.
+bool pitch_fits(long long pitch, int A) { return pitch >= A && pitch <= 1LL << 31; }
+
 // What both losses ask of their rows; fills the shared part of r.
 int take_rows(const char* who, const ob200_policy_rows* p, Rows* r) {
     if (!p) return set_error(OB200_ERR_INVALID, "%s: null argument", who);
     if (p->dtype != OB200_DTYPE_BF16 && p->dtype != OB200_DTYPE_F16 && p->dtype != OB200_DTYPE_F32)
         return set_error(OB200_ERR_INVALID, "%s: bad dtype %d", who, p->dtype);
     if (p->n < 0 || p->n_actions < 1) return set_error(OB200_ERR_INVALID, "%s: bad size (n %d, n_actions %d)", who, p->n, p->n_actions);
+    if (p->n_actions > (1 << 30)) return set_error(OB200_ERR_TOO_LARGE, "%s: over 2^30 actions", who);
     if (p->n == 0) return OB200_OK;
     const int es = elem_bytes(p->dtype);
     if (!p->logits || !p->grad) return set_error(OB200_ERR_INVALID, "%s: null logits or grad", who);
-    if (p->logits_pitch < p->n_actions || p->grad_pitch < p->n_actions)
-        return set_error(OB200_ERR_INVALID, "%s: a pitch is below n_actions", who);
+    if (!pitch_fits(p->logits_pitch, p->n_actions) || !pitch_fits(p->grad_pitch, p->n_actions))
+        return set_error(OB200_ERR_INVALID, "%s: a pitch is below n_actions, or above 2^31", who);
     if (((uintptr_t)p->logits | (uintptr_t)p->grad) % es || ((uintptr_t)p->legal_bits | (uintptr_t)p->row_weight | (uintptr_t)p->loss) % 4 || (uintptr_t)p->stats % 16)
         return set_error(OB200_ERR_INVALID, "%s: a pointer is not aligned", who);
     if (p->legal_bits && p->mask_words < (p->n_actions + 31) / 32)
@@ -76,7 +80,7 @@ int ob200_launch_policy_loss_search(const ob200_policy_rows* rows, const void* t
     if (target_kind != OB200_TARGET_VISITS && target_kind != OB200_TARGET_PROBS)
         return set_error(OB200_ERR_INVALID, "%s: bad target_kind %d", who, target_kind);
     if (rows->n > 0) {
-        if (!target || (uintptr_t)target % 4 || target_pitch < r.A)
+        if (!target || (uintptr_t)target % 4 || !pitch_fits(target_pitch, r.A))
             return set_error(OB200_ERR_INVALID, "%s: target is null, not aligned, or its pitch is below n_actions", who);
         if (rows_meet(r.grad, r.g_pitch, elem_bytes(rows->dtype), target, target_pitch, 4, r.n, r.A))
             return set_error(OB200_ERR_INVALID, "%s: grad overlaps target", who);
@@ -102,7 +106,7 @@ int ob200_launch_policy_loss_clipped(const ob200_policy_rows* rows, const int32_
             return set_error(OB200_ERR_INVALID, "%s: action, old_logp or advantage is null or not aligned", who);
         if (ref_logits) {
             const int es = elem_bytes(rows->dtype);
-            if ((uintptr_t)ref_logits % es || ref_pitch < r.A)
+            if ((uintptr_t)ref_logits % es || !pitch_fits(ref_pitch, r.A))
                 return set_error(OB200_ERR_INVALID, "%s: ref_logits is not aligned or its pitch is below n_actions", who);
             if (rows_meet(r.grad, r.g_pitch, es, ref_logits, ref_pitch, es, r.n, r.A))
                 return set_error(OB200_ERR_INVALID, "%s: grad overlaps ref_logits", who);

@@ -261,6 +261,7 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
         live = join(some, true) != 0.f;
     }
     if (live)
+#pragma unroll 4
         for (int j = tid; j < r.A; j += threads)
             if (legal(bits, j)) {
                 const float v = to_f32(z[j]);
@@ -274,6 +275,7 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
     live = live && q.m != -kInf;
     if (KIND != kClippedRef || q.c == -kInf) q.c = 0.f;
     if (live)
+#pragma unroll 4
         for (int j = tid; j < r.A; j += threads)
             if (legal(bits, j)) {
                 const float d = to_f32(z[j]) - q.m, e = ex2(d * kLog2e), dl = fmaxf(d, kLow), y = second(j);
@@ -289,6 +291,7 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
     RowOut out;
     live = row_result<KIND>(r, q, w, KIND == kSearch ? 0.f : r.old_logp[row], KIND == kSearch ? 0.f : r.advantage[row], &g, &out) && live;
     if (tid == 0) put_out(r, row, live, out);
+#pragma unroll 4
     for (int j = tid; j < r.A; j += threads) {
         float o = 0.f;
         if (live && legal(bits, j)) {
@@ -309,19 +312,34 @@ __device__ __noinline__ void careful_row(const PolicyRows& r, long long row) {
     plain_row<T, KIND>(r, row, threadIdx.x % 32, 32, [](float v, bool is_max) { return is_max ? warp_max_nan(v) : team_sum(v); });
 }
 
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A cluster of eight CTAs a row: 148 rows of 400,000 fp32 actions with a reference 499 us, one row 76 (a CTA a row: 1,397 and 510).
+constexpr int kLongCtas = 8;
 template <typename T, int KIND>
-__global__ void __launch_bounds__(512)
+__global__ void __cluster_dims__(kLongCtas) __launch_bounds__(512)
 policy_long_rows_kernel(const __grid_constant__ PolicyRows r) {
-    __shared__ float part[2][16];
+    __shared__ float part[2][kLongCtas * 16];
+    uint32_t cta;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     int turn = 0;
-    plain_row<T, KIND>(r, blockIdx.x, threadIdx.x, 512, [&](float v, bool is_max) {
+    cluster_barrier();                           // the others write into this CTA's shared memory
+    plain_row<T, KIND>(r, blockIdx.x / kLongCtas, (int)cta * 512 + threadIdx.x, kLongCtas * 512, [&](float v, bool is_max) {
         v = is_max ? warp_max_nan(v) : team_sum(v);
-        if (threadIdx.x % 32 == 0) part[turn][threadIdx.x / 32] = v;
-        __syncthreads();
-        v = part[turn][threadIdx.x % 16];
+        if (lane < kLongCtas) {
+            uint32_t there;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(ptx::smem_u32(&part[turn][cta * 16 + warp])), "r"(lane));
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
+        }
+        cluster_barrier();
+        const float *p = part[turn] + lane, a = p[0], b = p[32], c = p[64], d = p[96];
         turn ^= 1;
-        return is_max ? warp_max_nan(v) : team_sum<16>(v);
+        return is_max ? warp_max_nan(max_nan(max_nan(a, b), max_nan(c, d))) : team_sum((a + b) + (c + d));
     });
+    cluster_barrier();
 }
 
 // ---- rows in shared memory ------------------------------------------------------------
@@ -895,9 +913,6 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
 }
 
 // ---- rows of a CTA or a cluster ----------------------------------------------------------
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // What a warp or a CTA found of a row, relative to its own largest logit m and reference logit c - or to 0 where it has no
 // ordinary one: its terms are 0 then.
 template <typename T>
@@ -1072,19 +1087,20 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
 constexpr int kSms = 148;
 constexpr int kMostShared = 208 * 1024;          // of a CTA; 227 KB less the kernels' own
 
-// Registers of a thread | SMs << 16, looked up once for each kernel; every device is of the same kind.
+// Registers of a thread | SMs << 16.  Looked up once for each kernel and device, where the kernel is also given its shared
+// memory.
+struct KernelFacts { std::atomic<int> of[64]; };
 template <typename Kernel>
-int kernel_facts(Kernel kernel, std::atomic<int>* known, int* facts) {
-    *facts = known->load(std::memory_order_acquire);
-    if (*facts) return OB200_OK;
+int kernel_facts(Kernel kernel, KernelFacts* known, int* facts) {
     int dev = 0, sms = 0;
-    cudaFuncAttributes a;
     OB200_CUDA_OK(cudaGetDevice(&dev));
+    if (dev < 64 && (*facts = known->of[dev].load(std::memory_order_acquire)) != 0) return OB200_OK;
+    cudaFuncAttributes a;
     OB200_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     OB200_CUDA_OK(cudaFuncGetAttributes(&a, kernel));
     OB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
     *facts = a.numRegs | sms << 16;
-    known->store(*facts, std::memory_order_release);
+    if (dev < 64) known->of[dev].store(*facts, std::memory_order_release);
     return OB200_OK;
 }
 // CTAs the device holds at once.
@@ -1098,7 +1114,7 @@ int resident_ctas(int facts, int threads, int smem) {
 template <typename T, int KIND, int LANES, bool ALIKE>
 int launch_warp_rows(const PolicyRows& r, const RowShape& sh, cudaStream_t st) {
     constexpr int R = 32 / LANES;
-    static std::atomic<int> known{0};
+    static KernelFacts known;
     auto kernel = policy_warp_rows_kernel<T, KIND, LANES, ALIKE>;
     int facts;
     if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
@@ -1111,7 +1127,7 @@ int launch_warp_rows(const PolicyRows& r, const RowShape& sh, cudaStream_t st) {
 
 template <typename T, int KIND, bool ALIKE>
 int launch_cta_rows(const PolicyRows& r, const RowShape& sh, int warps, int ctas, cudaStream_t st) {
-    static std::atomic<int> known{0};
+    static KernelFacts known;
     auto kernel = policy_cta_rows_kernel<T, KIND, ALIKE>;
     int facts;
     if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
@@ -1183,7 +1199,8 @@ int launch_shape(const PolicyRows& r, cudaStream_t st) {
             return launch_cta_rows<T, KIND, ALIKE>(r, sh, warps > most ? most : warps, ctas, st);
         }
     }
-    policy_long_rows_kernel<T, KIND><<<(unsigned)r.n, 512, 0, st>>>(r);
+    if ((long long)r.n * kLongCtas > 0x7fffffffLL) return set_error(OB200_ERR_TOO_LARGE, "policy loss: %d rows of %d actions", r.n, r.A);
+    policy_long_rows_kernel<T, KIND><<<(unsigned)(r.n * kLongCtas), 512, 0, st>>>(r);
     OB200_LAUNCHED("policy_long_rows_kernel");
     return OB200_OK;
 }

@@ -125,7 +125,7 @@ def half_step(dt):
 
 
 SIZES = [(1, 1), (1, 2), (5, 31), (4, 32), (9, 33), (3, 127), (300, 225), (37, 362), (3, 511), (3, 513), (4, 1023), (3, 1024),
-         (5, 1025), (3, 2049), (70, 4672), (2, 8191), (2, 8193), (1, 16384), (2, 32769), (1, 65536), (1, 65537), (2, 150001)]
+         (5, 1025), (3, 2049), (70, 4672), (2, 8191), (2, 8193), (1, 16384), (2, 32769), (1, 65536), (1, 65537), (2, 150001), (3, 300007)]
 
 
 @pytest.mark.parametrize("n,A", SIZES)
@@ -270,7 +270,7 @@ def test_gradient_against_differences(api, A, kind):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("A", [33, 225, 4672, 40000])
+@pytest.mark.parametrize("A", [33, 225, 4672, 40000, 300007])
 def test_lowest_values_and_infinities(api, dt, A):
     import torch
     T = dtype_of(dt)
@@ -308,7 +308,7 @@ def test_all_rows_left_out_and_no_rows(api):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("A", [225, 1000, 4672, 32768, 70000])
+@pytest.mark.parametrize("A", [225, 1000, 4672, 32768, 70000, 300007])
 def test_gradient_in_place(api, dt, A):
     import torch
     g = torch.Generator(device="cuda")
@@ -345,6 +345,41 @@ def test_optional_outputs_streams_and_graph(api):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(grad, api.policy_loss_search(z, t)[1])
+
+
+@pytest.mark.parametrize("A", [225, 1030, 40000])
+def test_many_rows_of_each_kind(api, A):
+    """More rows than teams: rows of weight 0, without a legal action, with a single one, at the lowest value alone, in turn,
+    against the definition in 64 bits for a few of each."""
+    import torch
+    n = 40000 if A == 225 else 3000 if A == 1030 else 700
+    g = torch.Generator(device="cuda")
+    g.manual_seed(A)
+    z = torch.randn((n, A), generator=g, device="cuda").mul_(3).bfloat16()
+    t = torch.rand((n, A), generator=g, device="cuda")
+    legal = torch.rand((n, A), generator=g, device="cuda") < 0.6
+    w = torch.ones(n, device="cuda")
+    kind = torch.arange(n, device="cuda") % 7
+    w[kind == 1] = 0
+    legal[kind == 2] = False
+    legal[kind == 3] = False
+    legal[kind == 3, A // 3] = True
+    z[kind == 4] = torch.finfo(torch.bfloat16).min
+    z[kind == 5] = -float("inf")
+    loss, grad, stats = api.policy_loss_search(z, t, pack(legal.cpu().numpy()), w, entropy_coef=0.1)
+    torch.cuda.synchronize()
+    for k in (1, 2, 5):
+        assert not loss[kind == k].any() and not grad[kind == k].any() and not stats[kind == k].any()
+    assert not grad[~legal].any()
+    rows = torch.cat([(kind == k).nonzero()[[0, 1, -1], 0] for k in (0, 3, 4, 6)])
+    z64 = np.where(kind.cpu().numpy()[rows.cpu().numpy(), None] == 4, 0.0, z[rows].double().cpu().numpy())      # all alike: the same policy
+    rl, rg, rs, terms = ref_search(z64, legal[rows].cpu().numpy(), t[rows].double().cpu().numpy(), np.ones(len(rows)), 0.1)
+    reach = 2 * np.abs(z64).max() + 1
+    D = relative_bound(A, reach)
+    half, least = half_step(torch.bfloat16)
+    assert (np.abs(grad[rows].double().cpu().numpy() - rg) <= 4 * D * terms + half * np.abs(rg) + least).all()
+    got = stats[rows].double().cpu().numpy()
+    assert (np.abs(got - rs)[:, :3] <= 4 * D * (1 + reach + np.abs(rs[:, :3]))).all()
 
 
 def test_more_rows_than_a_grid_dimension(api):

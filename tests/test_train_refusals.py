@@ -41,6 +41,8 @@ def test_policy_rows_refused(api, bad):
 
 def test_policy_losses_refused(api):
     r = rows(api)
+    assert search(api, rows(api, n_actions=(1 << 30) + 1, logits_pitch=1 << 31, grad_pitch=1 << 31)) == 7
+    assert search(api, rows(api, logits_pitch=(1 << 31) + 1)) == api.ERR_INVALID
     assert search(api, None) == clipped(api, None) == api.ERR_INVALID
     assert search(api, r, target=None) == search(api, r, target=0x2000002) == search(api, r, pitch=224) == search(api, r, kind=2) == api.ERR_INVALID
     assert search(api, r, target=0x900000 + 64) == api.ERR_INVALID
