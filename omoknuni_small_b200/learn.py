@@ -120,14 +120,16 @@ class HeadLearner:
     def _backward(self, logits, grad, value, outcome, weight):
         """Gradients of both heads into the flat buffer; the value's loss, row by row."""
         torch = self.torch
-        off = value.detach() - outcome
+        # a row of weight 0 may hold anything as its outcome
+        off = torch.where(weight != 0, value.detach() - outcome, 0.0)
         self.flat_grad.zero_()
         torch.autograd.backward([logits, value], [grad, 2.0 * self.value_coef * weight * off])
         return self.value_coef * weight * off * off
 
     def _update(self, lr):
-        self.norm.run(self.max_norm)
+        norm = self.norm.run(self.max_norm)
         self.opt.step(lr, grad_scale=self.norm.clip)
+        return norm.clone()                        # the next step writes the plan's own again
 
     def _weight(self, n, row_weight):
         torch = self.torch
@@ -142,8 +144,8 @@ class HeadLearner:
             logits, value = self.heads(self.features(history, n_hist, to_move))
             loss, grad, stats = capi.policy_loss_search(logits.detach(), target, legal_bits, w, self.entropy_coef)
             value_loss = self._backward(logits, grad, value, outcome, w)
-            self._update(lr)
-        return loss, value_loss, stats, self.norm.out
+            norm = self._update(lr)
+        return loss, value_loss, stats, norm
 
     def step_clipped(self, history, n_hist, to_move, action, old_logp, advantage, outcome, legal_bits=None, row_weight=None, clip=0.2,
                      kl_coef=0.0, lr=1e-3):
@@ -160,8 +162,8 @@ class HeadLearner:
             loss, grad, stats = capi.policy_loss_clipped(logits.detach(), action, old_logp, advantage, legal_bits, ref, w, clip, clip, kl_coef,
                                                          self.entropy_coef)
             value_loss = self._backward(logits, grad, value, outcome, w)
-            self._update(lr)
-        return loss, value_loss, stats, self.norm.out
+            norm = self._update(lr)
+        return loss, value_loss, stats, norm
 
     def fit(self, records, steps, batch=512, lr=1e-3, seed=0):
         """`steps` steps of step_search on positions drawn from self-play records.  Returns the mean losses [steps, 2]."""
@@ -175,7 +177,7 @@ class HeadLearner:
             b = {k: torch.from_numpy(v).to(self.device) for k, v in b.items()}
             loss, value_loss, _, _ = self.step_search(b["history"], b["n_hist"], b["to_move"], b["target"], b["outcome"], b["legal_bits"], lr=lr)
             seen.append(torch.stack([loss.sum(), value_loss.sum()]))
-        return torch.stack(seen).cpu().numpy()
+        return torch.stack(seen).cpu().numpy() if seen else np.zeros((0, 2), np.float32)
 
     def weights(self):
         """Every tensor of the network under the reference's names, the heads as they are now (numpy float32)."""

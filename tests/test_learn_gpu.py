@@ -119,6 +119,31 @@ def test_records_to_a_new_handle(api, bits):
     assert np.abs(got - logits).max() <= 1e-4 * (1 + np.abs(logits).max()) and np.abs(v - value).max() <= 1e-4
 
 
+def test_rows_that_fill_up_a_batch(api):
+    """Rows of weight 0 change nothing whatever stands in their targets and outcomes; what a step returned stays as it was."""
+    import torch
+    _, _, a = make(api)
+    _, _, b = make(api)
+    clean, _ = batch(40)
+    fill = {k: v.clone() for k, v in clean.items()}
+    fill["outcome"][24:] = float("nan")
+    fill["visits"][24:] = -1
+    fill["legal_bits"][24:] = 0
+    w = torch.full((40,), 1.0 / 24, device="cuda")
+    w[24:] = 0
+    args = ("history", "n_hist", "to_move", "visits", "outcome", "legal_bits")
+    first = a.step_search(*[clean[k] for k in args], row_weight=w, lr=1e-3)
+    kept = [t.clone() for t in first]
+    got = b.step_search(*[fill[k] for k in args], row_weight=w, lr=1e-3)
+    assert all(torch.isfinite(x).all() and torch.equal(x, y) for x, y in zip(got, first))
+    assert not got[0][24:].any() and not got[1][24:].any() and first[0][:24].all()
+    assert all(torch.equal(p, b.params[k]) for k, p in a.params.items())
+    a.step_search(*[clean[k] for k in args], row_weight=w, lr=1e-3)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(first, kept))
+    assert a.fit([{"moves": [0], "winner": 0, "policies": [[1.0] * 225]}], steps=0).shape == (0, 2)
+
+
 def test_refusals(api):
     import torch
     net, w, learner = make(api, B=16)
