@@ -812,7 +812,7 @@ class AdamW:
 
     def step(self, lr, step=None, grad_scale=None):
         """One step.  lr: a number, or a float32 scalar on the device; step: 1 for the first one (default: counted here), or an
-        int32 scalar on the device - for captured graphs; grad_scale: a float32 scalar on the device that multiplies every
+        int32 scalar on the device - for captured graphs, nothing is changed while it is below 1; grad_scale: a float32 scalar on the device that multiplies every
         gradient (GradNorm.clip); when it is not finite weights and states stay as they are, while the count goes on."""
         import torch
         c = self.cfg

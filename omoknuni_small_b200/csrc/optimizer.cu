@@ -223,7 +223,9 @@ adamw_kernel(const __grid_constant__ Table<N> t, const __grid_constant__ Step k)
     const float lr = k.lr_device ? *k.lr_device : k.lr;
     float rate = k.rate, root = k.root;
     if (k.step_device) {
-        const double step = (double)*k.step_device;
+        const int32_t at = *k.step_device;
+        if (at < 1) return;                  // as the host's count is refused
+        const double step = (double)at;
         rate = (float)(1.0 / (1.0 - pow(k.beta1_d, step)));
         root = (float)(1.0 / sqrt(1.0 - pow(k.beta2_d, step)));
     }

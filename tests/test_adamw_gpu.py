@@ -311,3 +311,83 @@ def test_captured_training_step(api):
         h["norm"].run(0.5)
         h["opt"].step(0.01 / (k + 1), grad_scale=h["norm"].clip)
     assert torch.allclose(h["w"], a["w"], rtol=0, atol=4 * 0.01 * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_device_step_below_one_changes_nothing(api, bits):
+    import torch
+    opt, pflat, mflat, vflat = make(api, ODD, "f32", "f32", bits, 0)
+    before = [bits_of(f).clone() for f in (pflat, mflat, vflat)]
+    step = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for k in (0, -3):
+        step.fill_(k)
+        opt.step(0.01, step=step)
+        assert all(torch.equal(bits_of(f), b) for f, b in zip((pflat, mflat, vflat), before))
+    step.fill_(1)
+    opt.step(0.01, step=step)
+    assert not torch.equal(bits_of(pflat), before[0])
+
+
+def test_plans_on_two_streams_and_in_two_graphs(api):
+    """Plans of their own at the same time, and one plan in two graphs and without one: each norm is the one it gives alone."""
+    import torch
+    torch.manual_seed(1)
+    lists = [[torch.randn(n + k, device="cuda") for n in (300000, 5, 70000) * 20] for k in (0, 1)]
+    plans = [api.GradNorm(gs) for gs in lists]
+    want = [p.run(1.0).clone() for p in plans]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in plans], [[], []]
+    for _ in range(20):
+        for s, p, out in zip(streams, plans, got):
+            with torch.cuda.stream(s):
+                out.append(p.run(1.0).clone())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for out, w in zip(got, want) for x in out)
+    graphs = []
+    for limit in (1.0, 2.0):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            plans[0].run(limit)
+    for i in (0, 1, 1, 0):
+        graphs[i].replay()
+        twice = plans[0].out.clone()
+        assert torch.equal(twice[:1], want[0][:1]) and abs(float(twice[1] / want[0][1]) - (1 + i)) <= 2.0 ** -22
+        assert torch.equal(plans[0].run(1.0), want[0])
+
+
+FIRST = """
+import torch
+from omoknuni_small_b200 import capi
+n = 6
+z = {A: torch.randn(n, A, device="cuda") for A in (225, 4672, 40000, 300007)}
+t = {A: torch.rand(n, A, device="cuda") for A in z}
+act, one = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.ones(n, device="cuda")
+p, g = [torch.ones(5000, device="cuda") for _ in range(2)]
+norm, opt = capi.GradNorm([g]), capi.AdamW([p], [g], state_bits=8)
+count = torch.zeros(1, dtype=torch.int32, device="cuda")
+def calls():
+    out = [x for A in z for x in capi.policy_loss_search(z[A], t[A])]
+    out += [x for A in z for x in capi.policy_loss_clipped(z[A], act, -one, one, ref_logits=t[A], kl_coef=0.1)]
+    norm.run(1.0)
+    count.add_(1)
+    opt.step(0.01, step=count, grad_scale=norm.clip)
+    return out
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+graph.replay()
+torch.cuda.synchronize()
+w = p.clone()
+assert float(norm.out[0]) > 1 and not (w == 1).any()
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+"""
+
+
+def test_first_call_of_a_process_is_captured(api):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
