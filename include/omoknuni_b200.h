@@ -682,7 +682,8 @@ int ob200_copy_to_host(void* dst_host, const void* src_device, int64_t bytes);
  * what they hold does not matter.
  * Matrices whose rows start at the same place within 16 bytes of each other's
  * (all contiguous ones from the usual allocators) are read and written 16 bytes
- * at a time, others element by element. */
+ * at a time, others element by element.  grad, loss and stats share no memory with
+ * each other or with an input, but for grad with logits as said below. */
 typedef struct ob200_policy_rows {
     const void* logits;         /* [n][logits_pitch] of dtype                     */
     const uint32_t* legal_bits; /* [n][mask_words] as ob200_tree_view, or NULL    */
@@ -765,7 +766,7 @@ typedef struct ob200_adamw_config {
                                    is not finite the call changes nothing         */
     const float* lr_device;     /* DEVICE, or NULL: used in place of lr           */
     const int32_t* step_device; /* DEVICE, or NULL: used in place of step (for
-                                   captured graphs)                               */
+                                   captured graphs).  Below 1 the call changes nothing */
 } ob200_adamw_config;
 
 /* One AdamW step over all tensors, for each element, in fp32:

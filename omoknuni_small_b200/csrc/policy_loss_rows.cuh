@@ -947,6 +947,9 @@ __device__ __forceinline__ Sums join_entries(const float (*entry)[8], int n) {
 // A CTA, or a cluster's CTAs, a row.  A warp's sums are relative to its own maxima and are joined by every warp at once, so
 // that a row costs one meeting of its warps, and one more before its slot takes the next row; while a CTA waits for its
 // copy the SM's others work.
+// (A run of the row for each warp to itself, copied in one, two or four pieces that refill as soon as their gradient has left,
+// and no second meeting: 4,096 x 32,768 bf16 199, 213, 225 us against 196, 2,048 x 4,672 25, 27, 29 against 21; what it costs
+// in instructions is more than the waits that it saves.)
 template <typename T, int KIND, bool ALIKE>
 __global__ void __launch_bounds__(256, 3)
 policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_constant__ RowShape sh) {

@@ -396,3 +396,28 @@ def test_more_rows_than_a_grid_dimension(api):
     torch.cuda.synchronize()
     assert abs(float(stats[0, 3]) - math.log(A)) < 1e-3 and 0 < float(stats[-1, 3]) < math.log(A) - 0.1
     assert not z[1:-1].any() and z[-1].any()
+
+
+@pytest.mark.parametrize("A", [225, 4672, 40000, 300007])
+def test_two_calls_at_once(api, A):
+    """Calls on two streams at the same time give what each gives alone."""
+    import torch
+    n = max(8, 4000000 // A)
+    torch.manual_seed(A)
+    zs = [torch.randn((n + k, A), device="cuda").bfloat16() for k in (0, 5)]
+    acts = [torch.randint(0, A, (z.shape[0],), device="cuda").int() for z in zs]
+    ones = [torch.ones(z.shape[0], device="cuda") for z in zs]
+
+    def call(k, out=None):
+        return api.policy_loss_clipped(zs[k], acts[k], -ones[k], ones[k], ref_logits=refs[k], kl_coef=0.1, out=out)
+    refs = [z.flip(1) for z in zs]
+    want = [call(0), call(1)]
+    outs = [[tuple(torch.zeros_like(x) for x in w) for _ in range(8)] for w in want]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in zs]
+    for i in range(8):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                call(k, outs[k][i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for w, rounds in zip(want, outs) for got in rounds for x, y in zip(got, w))
