@@ -702,7 +702,7 @@ typedef struct ob200_policy_rows {
 } ob200_policy_rows;
 
 #define OB200_TARGET_VISITS 0   /* int32 visit counts                             */
-#define OB200_TARGET_PROBS 1    /* fp32, any positive scale                       */
+#define OB200_TARGET_PROBS 1    /* fp32, any scale: sums from 1e-37 to 8e37       */
 
 /* Cross entropy with the search's visit distribution:
  *   pi = target / sum of target over the legal actions,  p = the policy,

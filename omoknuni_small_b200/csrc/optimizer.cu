@@ -23,6 +23,7 @@ constexpr int kBlock = 256;              // elements that share the scales of 8-
 template <int BITS> constexpr int kThreads = BITS == 8 ? 128 : 256;
 template <int BITS> constexpr int kChunk = 2048;
 template <typename G> constexpr int kNormChunk = 1024 * (16 / (int)sizeof(G));    // of a CTA's turn of the norm: 64 bytes a thread
+                                         // (24.5 M bf16, 4.2 M fp32: 14.2, 6.5 us; 32 bytes 13.9, 7.2; 128 and half the CTAs 15.8, 6.5)
 constexpr float kE4m3Max = 448.f, kE4m3Least = 0x1p-9f, kScaleFloor = 0x1p-110f;
 constexpr int kNormCtas = 1184;          // partial sums of the norm: eight CTAs per SM
 

@@ -10,7 +10,7 @@
 //   clipped term: d/dz_j = k ([j = action] - p_j),  k = -advantage r or 0
 // so a gradient is p_j (k0 + kz d_j + kd (d_j - d'_j)) plus a term of the action or of the target.
 //
-// Rows are worked on in shared memory, where bulk copies have brought them while the rows before were worked on: once for
+// Rows are worked on in shared memory, where bulk copies bring them while an SM's other teams work on theirs: once for
 // the maximum (where actions that do not count are replaced by a lowest value, so that the other passes ask no mask), once
 // for the sums, once for the gradient, which leaves in 16-byte stores.  Every matrix is read from memory once and the
 // gradient written once.  Next to memory, instructions are what bounds it: at 6.5 TB/s an SM has 33 thread instructions
@@ -18,7 +18,7 @@
 // instruction), the packed 16-bit maximum, and few threads a row, each with many actions:
 //   policy_warp_rows_kernel   short rows: 8, 16 or 32 lanes a row, so that what a row costs besides its actions is paid
 //                             once for up to four of them
-//   policy_cta_rows_kernel    the others: a CTA or the CTAs of a cluster a row, one warp copying ahead, one joining sums
+//   policy_cta_rows_kernel    the others: a CTA or the CTAs of a cluster a row
 //   policy_long_rows_kernel   rows beyond the shared memory of eight CTAs, three times through device memory
 #pragma once
 #include "common.h"
