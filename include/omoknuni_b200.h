@@ -771,12 +771,13 @@ typedef struct ob200_adamw_config {
 
 /* One AdamW step over all tensors, for each element, in fp32:
  *   g = grad * grad_scale
- *   m = beta1 * m + ((1 - beta1) * g),   v = beta2 * v + ((1 - beta2) * (g * g))     (fused multiply-adds)
+ *   m = beta1 * m + (1 - beta1) * g,   v = beta2 * v + (1 - beta2) * (g * g)     (each product and sum rounded)
  *   param = param * (1 - lr * weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
  * param is rounded once to its type; updates smaller than half a step of a
  * 16-bit type are lost, so keep fp32 weights where that matters.
  * state_bits 8: each run of 256 elements of a tensor shares an fp32 scale,
- * max / 448 (maxima below 2^-110 count as 2^-110): the first moment is held as
+ * max * (1 / 448) (maxima below 2^-110 count as 2^-110; a value times
+ * (1 / max) * 448, each rounded, becomes the code): the first moment is held as
  * e4m3 times its scale, the second as the square of (e4m3 times its scale), a
  * value above 0 never becoming 0.  The step itself uses m and v before they are
  * rounded.  Zeroed codes and scales are the state before the first step.

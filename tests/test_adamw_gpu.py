@@ -155,11 +155,10 @@ def quantise(x, root):
     b[:n] = x
     b = b.view(-1, 256)
     top = b.abs().amax(1, keepdim=True).clamp_min(2.0 ** -110)
-    q = b * (torch.full_like(top, 448.0) / top)
+    q = b * (top.reciprocal() * 448.0)
     if root:
         q = torch.where((b > 0) & (q < 2.0 ** -9), torch.full_like(q, 2.0 ** -9), q)
-    # by a tensor: a division by a number is a product with its rounded reciprocal in torch
-    return q.to(torch.float8_e4m3fn).view(torch.uint8).reshape(-1)[:n], (top / torch.full_like(top, 448.0)).view(-1)
+    return q.to(torch.float8_e4m3fn).view(torch.uint8).reshape(-1)[:n], (top * float(np.float32(1.0) / np.float32(448.0))).view(-1)
 
 
 def dequantise(q, scale):
@@ -191,10 +190,8 @@ def test_adamw_8_codes_are_exact(api, p_dt, g_dt, shift):
             g = opt.grads[i].float()
             m = dequantise(st["exp_avg"][i], st["exp_avg_scale"][i])
             v = dequantise(st["exp_avg_sq"][i], st["exp_avg_sq_scale"][i]).square()
-            # fused multiply-adds: in 64 bits the product is exact, and the sum's second rounding moves none of these values
-            b1, b2 = float(np.float32(0.9)), float(np.float32(0.999))
-            m = (m.double() * b1 + (g * (1.0 - 0.9)).double()).float()
-            v = (v.double() * b2 + ((g * g) * (1.0 - 0.999)).double()).float()
+            m = m * 0.9 + g * (1.0 - 0.9)
+            v = v * 0.999 + (g * g) * (1.0 - 0.999)
             mq, msc = quantise(m, False)
             vq, vsc = quantise(v.sqrt(), True)
             assert torch.equal(opt.state["exp_avg_scale"][i], msc) and torch.equal(opt.state["exp_avg_sq_scale"][i], vsc), i
