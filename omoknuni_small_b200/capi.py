@@ -730,6 +730,16 @@ def _same_kind(tensors, what):
     return _train_dtype(first.dtype, what), first.device
 
 
+def _cleared(make, device, what):
+    """make() - zeroed tensors that a plan keeps - done when this returns, so that the plan may run on any stream."""
+    import torch
+    with torch.cuda.device(device):
+        _require(not torch.cuda.is_current_stream_capturing(), "%s: a plan is made before a graph is captured, not in it", what)
+        made = make()
+        torch.cuda.current_stream().synchronize()
+    return made
+
+
 class GradNorm:
     """2-norm over a fixed list of gradients and the factor that clips it (ob200_launch_grad_norm).  run(max_norm) fills
     and returns `out` (float32 [2] on the device: norm, factor); `clip` is the factor as AdamW.step takes it.  The plan
@@ -741,11 +751,12 @@ class GradNorm:
         _require(len(self.grads) > 0, "GradNorm: no gradients")
         self.dtype, self.device = _same_kind(self.grads, "grad")
         _require(self.device.type == "cuda", "the tensors are not on a CUDA device (there is no CPU path)")
-        self.out = torch.zeros(2, dtype=torch.float32, device=self.device) if out is None else out
+        count = int(lib().ob200_grad_norm_workspace_bytes()) // 8
+        self.out, self.workspace = _cleared(lambda: (torch.zeros(2, dtype=torch.float32, device=self.device) if out is None else out,
+                                                     torch.zeros(count, dtype=torch.float64, device=self.device)), self.device, "GradNorm")
         _require(self.out.dtype == torch.float32 and self.out.device == self.device and tuple(self.out.shape) == (2,)
                  and self.out.is_contiguous(), "GradNorm: out is float32 [2] on the gradients' device")
         self.clip = self.out[1:]
-        self.workspace = torch.zeros(int(lib().ob200_grad_norm_workspace_bytes()) // 8, dtype=torch.float64, device=self.device)
         self.table = (TrainTensor * len(self.grads))()
         for e, g in zip(self.table, self.grads):
             e.grad, e.numel = g.data_ptr(), g.numel()
@@ -789,8 +800,8 @@ class AdamW:
         def size(p, per):
             return (p.numel() + per - 1) // per
         if state is None:
-            state = {k: [torch.zeros(size(p, per), dtype=torch.uint8 if dt == torch.float8_e4m3fn else dt, device=self.device).view(dt)
-                         for p in self.params] for k, (dt, per) in keys.items()}
+            state = _cleared(lambda: {k: [torch.zeros(size(p, per), dtype=torch.uint8 if dt == torch.float8_e4m3fn else dt, device=self.device).view(dt)
+                                          for p in self.params] for k, (dt, per) in keys.items()}, self.device, "AdamW")
         self.state = {k: list(state[k]) if k in state else None for k in keys}
         for k, (dt, per) in keys.items():
             _require(self.state[k] is not None and len(self.state[k]) == n, "AdamW: state %s: a tensor for each param is wanted", k)

@@ -388,3 +388,27 @@ def test_first_call_of_a_process_is_captured(api):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_plans_are_made_outside_captures_and_run_on_any_stream(api):
+    import torch
+    p, g = [torch.ones(70000, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g.add_(0)
+        with pytest.raises(api.Error):
+            api.GradNorm([g])
+        with pytest.raises(api.Error):
+            api.AdamW([p], [g])
+    side = torch.cuda.Stream()
+    big = torch.empty(1 << 28, device="cuda")
+    for k in range(3):
+        big.fill_(k)                                # keeps the stream of the plans busy
+        norm, opt = api.GradNorm([g]), api.AdamW([p], [g], state_bits=8)
+        with torch.cuda.stream(side):
+            got = norm.run(1.0)
+            opt.step(0.0, grad_scale=norm.clip)
+        side.synchronize()
+        assert abs(float(got[0]) - math.sqrt(70000.0)) <= 2.0 ** -20 * 265 and float(opt.state["exp_avg"][0].float().min()) == 448
+        assert float(p.min()) == 1 == float(p.max())
