@@ -891,6 +891,7 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && live;
         if (tid == 0 && is && !apart) put_out(r, row, live, out);
         T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
+        __syncwarp();                            // the gradient may take the place of the action's logit
         if (!apart) pass_grad<T, KIND, ALIKE, U, (LANES < 32)>(r, p, tid, LANES, live, g, act_e, grad);
         if (ALIKE) {
             // the slot's next copy comes behind what was read and written here
@@ -1026,11 +1027,12 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             const bool some = __any_sync(~0u, pass_max<T, KIND, ALIKE, U, false>(r, row, p, threadIdx.x, threads, &top_z, &top_x));
             const float top = warp_max_nan(word_top<T>(top_z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
             __syncwarp();
-            // the action's logit: of a cluster, by the warp that has its vector
+            // The action's logit, by the warp that has its vector and ahead of the meeting: behind it the others may find the
+            // gradient in its place.
             const int act_at = KIND != kSearch && act_e >= v0 * V && act_e < p.v1 * V && (!r.bits || (load_word(p.ms + 4 * ((act >> 5) - p.mask_first)) >> (act & 31)) & 1u)
                                    ? act_e - v0 * V : -1;
             float za = -kInf;
-            if (KIND != kSearch && ctas > 1 && act_at >= 0 && act_at / V % threads / 32 == warp) za = to_f32(in_shared<const T>(p.zs)[act_at]);
+            if (KIND != kSearch && act_at >= 0 && act_at / V % threads / 32 == warp) za = to_f32(in_shared<const T>(p.zs)[act_at]);
             Sums q;
             q.m = base_of<T>(top);
             q.c = KIND == kClippedRef ? base_of<T>(top_ref) : 0.f;
@@ -1041,7 +1043,7 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             float* const mine = all[cta * warps + warp];
             if (ctas == 1) {
                 if (lane < 4) mine[2 + lane] = sum;
-                else if (lane == 4) { mine[0] = top; mine[1] = top_ref; mine[6] = -kInf; mine[7] = some ? 1.f : 0.f; }
+                else if (lane == 4) { mine[0] = top; mine[1] = top_ref; mine[6] = za; mine[7] = some ? 1.f : 0.f; }
                 __syncthreads();
             } else {
                 const float s = __shfl_sync(~0u, sum, 0), t = __shfl_sync(~0u, sum, 1), a = __shfl_sync(~0u, sum, 2), b = __shfl_sync(~0u, sum, 3);
@@ -1054,7 +1056,6 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
                 cluster_barrier();
             }
             q = join_entries<T, KIND>(all, (int)ctas * warps);
-            if (KIND != kSearch && ctas == 1 && act_at >= 0) q.za = to_f32(in_shared<const T>(p.zs)[act_at]);
             const bool legal_one = __any_sync(~0u, lane < (int)ctas * warps && all[lane][7] != 0.f);      // else the row is left out
             apart = legal_one && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2));
             live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && legal_one;
