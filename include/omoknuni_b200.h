@@ -476,7 +476,11 @@ int ob200_net_forward_device(ob200_net* net, const void* input_board_tensor, int
  * up to 15x15) the tower kernel writes its own input planes from the histories -
  * no encoder launch and no input tensor in device memory; on the other paths the
  * encoder kernel runs first.  Results are those of ob200_launch_encode_gomoku +
- * ob200_net_forward_device. */
+ * ob200_net_forward_device.
+ * A handle has one set of activation buffers.  The host-buffer calls, searches and
+ * ob200_net_tower_copy_device are ordered with each other; the calls that take a
+ * stream (these two and ob200_net_tower_device) run on it as they come: order
+ * streams that use one handle, and wait before a host-buffer call or a search. */
 int ob200_net_forward_gomoku_device(ob200_net* net, const int16_t* history, const uint8_t* n_hist,
                                     const uint8_t* to_move, int32_t B, float* policy_out,
                                     float* value_out, int32_t out_kind, ob200_stream stream);
@@ -496,6 +500,14 @@ int32_t ob200_net_debug_tower_path(ob200_net* net);
  * For measurement and for callers that run their own heads. */
 int ob200_net_tower_device(ob200_net* net, const void* input_board_tensor, int32_t B,
                            ob200_stream stream);
+/* The same, its result copied into caller-owned memory: DEVICE tower_out, a board
+ * tensor of B boards and `filters` channels.  Tower and copy come behind what the
+ * host-buffer calls of the handle have enqueued, and what they and searches enqueue
+ * afterwards comes behind the copy, whatever `stream` is: the call for a learner
+ * whose handle also answers and searches.  `stream` must not be capturing
+ * (OB200_ERR_STATE). */
+int ob200_net_tower_copy_device(ob200_net* net, const void* input_board_tensor, int32_t B, void* tower_out,
+                                ob200_stream stream);
 /* The value head alone, for callers that must never allocate.  (No counterpart in
  * the reference: its value head runs inside ResNetModel::forward on libtorch's
  * caching allocator.)  Meant for search threads in the middle of a self-play loop
@@ -630,7 +642,9 @@ void ob200_search_destroy(ob200_search* s);
 /* One move for every tree.  HOST buffers.  moves[t * moves_stride + i], i in
  * [0, n_moves[t]): the game so far (BLACK first), legal and unfinished.
  * pi_out [n_trees][225]: visit counts -> (n / n_max)^(1/T) normalised, one-hot
- * argmax for temperature < 0.01; visits_out [n_trees][225] may be NULL. */
+ * argmax for temperature < 0.01; visits_out [n_trees][225] may be NULL.  Until it
+ * returns the search has the network's handle to itself: calls on it from other
+ * threads wait. */
 int ob200_search_run(ob200_search* s, const int16_t* moves, const int32_t* n_moves, int32_t moves_stride,
                      float temperature, float* pi_out, int32_t* visits_out, ob200_search_stats* stats);
 /* Test hooks: device pointers of the search's tree view and node counter, and a

@@ -157,6 +157,7 @@ SIGNATURES = {
     "ob200_net_debug_tower_output": (C.c_void_p, [C.c_void_p]),
     "ob200_net_debug_tower_path": (C.c_int32, [C.c_void_p]),
     "ob200_net_tower_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+    "ob200_net_tower_copy_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
     "ob200_net_input_tensor_channels": (C.c_int32, [C.c_void_p]),
     "ob200_net_value_head_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
     "ob200_value_head_noalloc_capacity": (C.c_int64, []),
@@ -496,6 +497,17 @@ class Net:
     def tower_device(self, input_bt, B):
         """The residual tower alone on a device input tensor (asynchronous)."""
         check(lib().ob200_net_tower_device(self.h, _ptr(input_bt), B, _stream()))
+
+    def tower_copy_device(self, input_bt, B, out=None):
+        """The same into memory of the caller's, ordered with the handle's own calls and searches whatever the current stream
+        is.  Returns the board tensor (int16 holding the 16-bit values; `out`: a tensor of that size to write into)."""
+        import torch
+        nbytes = int(lib().ob200_board_tensor_bytes(self.board_size, B, self.cfg.filters))
+        if out is None:
+            out = torch.empty(nbytes // 2, dtype=torch.int16, device=torch.device("cuda", self.cfg.device))
+        assert out.is_contiguous() and out.numel() * out.element_size() == nbytes
+        check(lib().ob200_net_tower_copy_device(self.h, _ptr(input_bt), B, _ptr(out), _stream()))
+        return out
 
     def tower_output_ptr(self):
         return lib().ob200_net_debug_tower_output(self.h)

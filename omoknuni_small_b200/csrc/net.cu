@@ -70,6 +70,7 @@ struct ob200_net {
     cudaStream_t copy_stream = nullptr;   // device -> host copies of results
     cudaStream_t in_stream = nullptr;     // host -> device copies of move histories, ahead of the batch that reads them
     cudaEvent_t planes_copied = nullptr;  // the planes staging buffer has been read by its host -> device copy
+    cudaEvent_t order = nullptr;          // between the handle's stream and another that uses the activation buffers
     float *d_planes = nullptr;
     float *h_planes = nullptr;
     size_t planes_capacity = 0;     // floats per staging buffer
@@ -275,6 +276,7 @@ void ob200_net_destroy(ob200_net* n) {
     if (n->stream) { cudaStreamSynchronize(n->stream); cudaStreamDestroy(n->stream); }
     if (n->copy_stream) { cudaStreamSynchronize(n->copy_stream); cudaStreamDestroy(n->copy_stream); }
     if (n->planes_copied) cudaEventDestroy(n->planes_copied);
+    if (n->order) cudaEventDestroy(n->order);
     if (n->in_stream) { cudaStreamSynchronize(n->in_stream); cudaStreamDestroy(n->in_stream); }
     for (auto& sl : n->slot) {
         if (sl.computed) cudaEventDestroy(sl.computed);
@@ -459,6 +461,7 @@ int ob200_net_finalize(ob200_net* n) {
     OB200_CUDA_OK(cudaStreamCreateWithFlags(&n->in_stream, cudaStreamNonBlocking));
     OB200_CUDA_OK(cudaEventCreateWithFlags(&n->planes_copied, cudaEventDisableTiming));
     OB200_CUDA_OK(cudaEventRecord(n->planes_copied, n->stream));
+    OB200_CUDA_OK(cudaEventCreateWithFlags(&n->order, cudaEventDisableTiming));
     OB200_CUDA_OK(cudaDeviceSynchronize());
     n->host.clear();
     n->finalized = true;
@@ -553,6 +556,13 @@ int tower_device(ob200_net* n, const void* input_bt, int B, int* out_buf, cudaSt
     }
     n->tower_out = n->act[x];
     *out_buf = x;
+    return OB200_OK;
+}
+
+// Work enqueued on `to` from here on comes behind what is on `from`.
+int order_streams(ob200_net* n, cudaStream_t from, cudaStream_t to) {
+    OB200_CUDA_OK(cudaEventRecord(n->order, from));
+    OB200_CUDA_OK(cudaStreamWaitEvent(to, n->order, 0));
     return OB200_OK;
 }
 
@@ -713,12 +723,19 @@ int enqueue_gomoku(ob200_net* n, int si, const int16_t* history, const uint8_t* 
 }  // namespace ob200
 
 namespace ob200 {
-// For the search loop: forward on device move histories, probabilities out, no locking
-// beyond the handle's (the search is the handle's only user while it runs).
+// For the search loop.  A search has the handle to itself: from begin to end it holds the handle's mutex, and its stream comes
+// behind what the other calls have enqueued (the activation buffers are the handle's).  At end its own work has completed.
+int net_begin_search(ob200_net* n, cudaStream_t st) {
+    if (!n || !n->finalized) return set_error(OB200_ERR_STATE, "search: the network is not finalised");
+    n->mu.lock();
+    const int rc = order_streams(n, n->stream, st);
+    if (rc) n->mu.unlock();
+    return rc;
+}
+void net_end_search(ob200_net* n) { n->mu.unlock(); }
+// Forward on device move histories, probabilities out; between begin and end.
 int net_forward_gomoku_for_search(ob200_net* n, const int16_t* hist, const uint8_t* nh, const uint8_t* tm, int B, float* policy,
                                   float* value, cudaStream_t st) {
-    if (!n || !n->finalized) return set_error(OB200_ERR_STATE, "search: the network is not finalised");
-    std::lock_guard<std::mutex> lk(n->mu);
     const GomokuInput g{hist, nh, tm};
     return forward_device(n, nullptr, B, policy, value, OB200_OUT_PROBS, st, &g);
 }
@@ -839,6 +856,34 @@ int ob200_net_tower_device(ob200_net* n, const void* input_board_tensor, int32_t
     OB200_CUDA_OK(cudaSetDevice(n->cfg.device));
     int x = 0;
     return tower_device(n, input_board_tensor, B, &x, as_stream(stream));
+}
+
+int ob200_net_tower_copy_device(ob200_net* n, const void* input_board_tensor, int32_t B, void* tower_out, ob200_stream stream) {
+    const char* who = "ob200_net_tower_copy_device";
+    if (!n || !input_board_tensor || !tower_out) return set_error(OB200_ERR_INVALID, "%s: null argument", who);
+    if (!n->finalized) return set_error(OB200_ERR_STATE, "%s: weights not finalised", who);
+    if (B < 1 || B > n->cfg.max_batch)
+        return set_error(OB200_ERR_TOO_LARGE, "%s: batch %d outside [1, max_batch %d]", who, B, n->cfg.max_batch);
+    std::lock_guard<std::mutex> lk(n->mu);
+    OB200_CUDA_OK(cudaSetDevice(n->cfg.device));
+    cudaStream_t st = as_stream(stream);
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    OB200_CUDA_OK(cudaStreamIsCapturing(st, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone)
+        return set_error(OB200_ERR_STATE, "%s: a replayed graph could not be ordered with the handle's other calls", who);
+    if (int rc = order_streams(n, n->stream, st)) return rc;
+    int x = 0;
+    int rc = tower_device(n, input_board_tensor, B, &x, st);
+    if (!rc) {
+        const BoardGeom g = board_geom(n->cfg.board_size, B);
+        const size_t cell = (size_t)n->cfg.filters * 2, boards = (size_t)(OB200_GUARD + g.P) * cell;
+        // behind the last board the handle's tensor holds what a larger batch left
+        if (cudaMemcpyAsync(tower_out, n->act[x], boards, cudaMemcpyDeviceToDevice, st) != cudaSuccess ||
+            cudaMemsetAsync((char*)tower_out + boards, 0, (size_t)g.PT * cell - boards, st) != cudaSuccess)
+            rc = set_error(OB200_ERR_CUDA, "%s: copying the tower's output failed", who);
+    }
+    const int after = order_streams(n, st, n->stream);       // on an error too: part of the tower may be under way
+    return rc ? rc : after;
 }
 
 int ob200_net_value_head_noalloc(ob200_net* n, const void* tower_board_tensor, int32_t B, float* value_out,

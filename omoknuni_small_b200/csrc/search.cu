@@ -556,6 +556,8 @@ expand_rows_kernel(ob200_tree_view t, const int32_t* __restrict__ paths, const i
 
 // Accessors of the network handle that the search needs (defined in net.cu).
 namespace ob200 {
+int net_begin_search(ob200_net* n, cudaStream_t st);
+void net_end_search(ob200_net* n);
 int net_forward_gomoku_for_search(ob200_net* n, const int16_t* hist, const uint8_t* nh, const uint8_t* tm, int B, float* policy,
                                   float* value, cudaStream_t st);
 const ob200_net_config* net_config(ob200_net* n);
@@ -748,6 +750,12 @@ int ob200_search_run(ob200_search* s, const int16_t* moves, const int32_t* n_mov
         nh[t] = (uint8_t)k; tm[t] = (uint8_t)((n & 1) ? 2 : 1); count[t] = n;
     }
     cudaStream_t st = s->stream;
+    if (int rc = net_begin_search(s->net, st)) return rc;
+    struct Taken {
+        ob200_search* s;
+        bool done = false;                   // the search's work has completed
+        ~Taken() { if (!done) cudaStreamSynchronize(s->stream); net_end_search(s->net); }
+    } taken{s};
     OB200_CUDA_OK(cudaMemcpyAsync(s->root_stones, stones.data(), stones.size() * 4, cudaMemcpyHostToDevice, st));
     OB200_CUDA_OK(cudaMemcpyAsync(s->root_hist, hist.data(), hist.size() * 2, cudaMemcpyHostToDevice, st));
     OB200_CUDA_OK(cudaMemcpyAsync(s->root_nh, nh.data(), T, cudaMemcpyHostToDevice, st));
@@ -865,6 +873,7 @@ int ob200_search_run(ob200_search* s, const int16_t* moves, const int32_t* n_mov
     int* errw = device_error_word();
     if (errw) OB200_CUDA_OK(cudaMemcpyAsync(&err, errw, 4, cudaMemcpyDeviceToHost, st));
     OB200_CUDA_OK(cudaStreamSynchronize(st));
+    taken.done = true;
     if (err) {
         cudaMemsetAsync(errw, 0, 4, st); cudaStreamSynchronize(st);
         return set_error(OB200_ERR_TIMEOUT, "a kernel gave up on a bounded wait (code %d) during the search", err);

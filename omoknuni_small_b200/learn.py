@@ -3,7 +3,7 @@
 Takes the place of one optimiser step of the reference's learner (alphazero_train.py,
 python/alphazero/alphazero_trainer.py: cross entropy with the search's policy plus squared error of the value, Adam) for
 the two heads; the tower stays as it is and runs on the handle's own kernels.  A step is: positions -> planes -> tower
-(capi.encode_gomoku, Net.tower_device), heads forward (PyTorch), loss and its gradient over the legal moves
+(capi.encode_gomoku, Net.tower_copy_device), heads forward (PyTorch), loss and its gradient over the legal moves
 (capi.policy_loss_search / policy_loss_clipped), heads backward (PyTorch), norm of the gradients and the weight update
 (capi.GradNorm, capi.AdamW).  weights() gives the whole network under the reference's names, for a new handle
 (capi.Net(...).load) and for checkpoint.write_flat.
@@ -44,15 +44,9 @@ def batch_of(positions, board_size):
     return dict(history=history, n_hist=n_hist, to_move=to_move, legal_bits=np.ascontiguousarray(bits), target=target, outcome=outcome)
 
 
-class _Memory:
-    """Device memory of the library as torch.as_tensor takes it."""
-
-    def __init__(self, ptr, count):
-        self.__cuda_array_interface__ = {"shape": (count,), "typestr": "<i2", "data": (ptr, False), "version": 3}
-
-
 class HeadLearner:
-    """One optimiser over the heads of `net` (a finalised capi.Net for Gomoku) whose tensors are `weights`.
+    """One optimiser over the heads of `net` (a finalised capi.Net for Gomoku) whose tensors are `weights`.  Steps run on
+    PyTorch's current stream and return without waiting; the handle may answer and search between them.
 
     state_bits: AdamW states in 32 or 8 bits.  max_norm: the gradients' norm is clipped to it.  value_coef: factor of the
     squared error of the value.  The heads as they are at the start are the reference of the KL term of step_clipped."""
@@ -93,13 +87,11 @@ class HeadLearner:
             raise capi.Error(capi.ERR_INVALID, f"HeadLearner: {n} positions, the handle takes {self.net.cfg.max_batch}")
         with torch.cuda.device(self.device):
             planes = capi.encode_gomoku(history, n_hist, to_move, S, self.net.cfg.input_channels, channels, self.net.tower_dtype)
-            self.net.tower_device(planes, n)
-            count = capi.board_positions(S, n) * self.F
-            raw = torch.as_tensor(_Memory(self.net.tower_output_ptr(), count), device=self.device)
+            raw = self.net.tower_copy_device(planes, n)      # the handle's own memory belongs to its next call
             t = raw.view(torch.float16 if self.net.tower_dtype == capi.DTYPE_F16 else torch.bfloat16)
             G, GP = capi.GUARD, S + 1
             x = t.as_strided((n, self.F, S, S), (GP * GP * self.F, 1, GP * self.F, self.F), G * self.F)
-            return x.float()                       # a copy: the next call writes the tower's output again
+            return x.float()
 
     def heads(self, x, params=None):
         """(logits [n, A], value [n]) of tower outputs, BatchNorm with its stored statistics."""
