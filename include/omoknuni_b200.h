@@ -737,9 +737,10 @@ int ob200_launch_policy_loss_search(const ob200_policy_rows* rows, const void* t
  * The gradient of the first term is that of r * advantage where it is not the
  * larger one, 0 elsewhere; an advantage of 0 contributes 0 whatever r is.
  * ref_logits may be NULL (KL = 0; kl_coef must then be 0).  KL becomes very large,
- * not infinite, where q gives no probability to an action that p gives some (and
- * infinite where q gives none to any).  A row whose action is outside
- * [0, n_actions) or not legal is left out. */
+ * not infinite, where q gives no probability to an action that p gives some.  Where
+ * q gives none to any legal action it is infinite, and without a gradient: that of
+ * the row is its other terms', and with kl_coef 0 so is the loss.  A row whose
+ * action is outside [0, n_actions) or not legal is left out. */
 int ob200_launch_policy_loss_clipped(const ob200_policy_rows* rows, const int32_t* action, const float* old_logp,
                                      const float* advantage, const void* ref_logits, int64_t ref_pitch,
                                      float clip_low, float clip_high, float kl_coef, float entropy_coef,

@@ -220,15 +220,17 @@ __device__ __forceinline__ bool row_result(const PolicyRows& r, const Sums& q, f
     const bool free = open <= held || open != open, none = adv == 0.f;
     const float surrogate = none ? 0.f : free ? open : held, k = none || !free ? 0.f : -open;
     float kl = 0.f, ud = 0.f;
+    g->kd = w * r.kl;
     if (KIND == kClippedRef) {
         ud = q.a * inv_s;
         kl = ud - (l2s - lg2(q.b)) * kLn2;
         if (kl != kl) ud = kl;
+        // The reference gives no legal action any probability: KL is infinite whatever p is, and has no gradient.
+        if (q.b == 0.f) { kl = kInf; ud = g->kd = 0.f; }
     }
     g->k0 = w * (-k - r.kl * ud - r.entropy * mean);
-    g->kd = w * r.kl;
     g->ka = w * k;
-    o->loss = w * (-surrogate + r.kl * kl - r.entropy * H);
+    o->loss = w * (-surrogate + (r.kl == 0.f && kl == kInf ? 0.f : r.kl * kl) - r.entropy * H);
     o->stats = make_float4(logp, ratio, kl, H);
     return q.za != -kInf;
 }
