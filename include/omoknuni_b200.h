@@ -687,8 +687,9 @@ int ob200_copy_to_host(void* dst_host, const void* src_device, int64_t bytes);
  * An action is legal when its bit is set (legal_bits NULL: all are); the policy
  * is the softmax over the legal actions, and what stands at other places
  * (infinities and NaN included) does not matter.  A logit of -inf is a
- * probability of 0; in sums over differences of logits (H, KL, cross entropy)
- * those below -1e30 count as -1e30.
+ * probability of 0; in sums over differences from the row's largest logit (H, KL,
+ * cross entropy, log p) those below -1e30 count as -1e30 (bf16: -1.5703125 * 2^99,
+ * its next value), whatever the type and the kernel.
  * A row is left out - loss, statistics and gradient are 0 - when its weight is 0
  * (its logits are then not read), when no legal action has a logit above -inf, or
  * for the reason its loss names.  A NaN or +inf logit of a legal action makes its

@@ -55,7 +55,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_inff();
-constexpr float kLow = -1e30f;          // differences below it count as it, so that products with a probability of 0 are 0
+// Differences below it count as it, so that products with a probability of 0 are 0.
+template <typename T> constexpr float kLow = -1e30f;
+template <> constexpr float kLow<__nv_bfloat16> = -0x1.92p99f;   // the value of bf16 next to it, which stands for it in a row (Lowest)
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -118,9 +120,11 @@ __device__ __forceinline__ f32x2 ex2_2(f32x2 v) {
 // ---- 16 bytes of a row ------------------------------------------------------------
 // The value that stands for logits that do not count, and for those below it: in every element of a word, and as fp32.
 // A row whose largest logit is below half of it is worked on separately (careful_row).
+// fp16 has no value so low that it could stand for a legal -inf: those stay, and threads that met one work with the passes
+// that look for them (FLOOR).
 template <typename T> struct Lowest;
-template <> struct Lowest<float> { static constexpr uint32_t kWord = 0xF149F2CAu; static constexpr float kValue = -1e30f; };
-template <> struct Lowest<__nv_bfloat16> { static constexpr uint32_t kWord = 0xF149F149u; static constexpr float kValue = -9.95e29f; };
+template <> struct Lowest<float> { static constexpr uint32_t kWord = 0xF149F2CAu; static constexpr float kValue = kLow<float>; };
+template <> struct Lowest<__nv_bfloat16> { static constexpr uint32_t kWord = 0xF149F149u; static constexpr float kValue = kLow<__nv_bfloat16>; };
 template <> struct Lowest<__half> { static constexpr uint32_t kWord = 0xFBFFFBFFu; static constexpr float kValue = -65504.f; };
 
 // Elements 2i and 2i + 1 of a vector of T as fp32.
@@ -132,7 +136,7 @@ __device__ __forceinline__ f32x2 elements(const uint32_t* v, int i) {
     return pair(f.x, f.y);
 }
 // The same less c (given as -c), in fp32: a 16-bit operand needs no conversion of its own.
-template <typename T>
+template <typename T, bool FLOOR = false>
 __device__ __forceinline__ f32x2 elements_less(const uint32_t* v, int i, f32x2 minus_c, float c) {
     if (sizeof(T) == 4) return add2(elements<T>(v, i), minus_c);
     float a, b;
@@ -140,6 +144,7 @@ __device__ __forceinline__ f32x2 elements_less(const uint32_t* v, int i, f32x2 m
         asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; sub.rn.f32.bf16 %0, l, %3; sub.rn.f32.bf16 %1, h, %3;}" : "=f"(a), "=f"(b) : "r"(v[i]), "f"(c));
     else
         asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; sub.rn.f32.f16 %0, l, %3; sub.rn.f32.f16 %1, h, %3;}" : "=f"(a), "=f"(b) : "r"(v[i]), "f"(c));
+    if (FLOOR) { a = max_nan(a, kLow<T>); b = max_nan(b, kLow<T>); }
     return pair(a, b);
 }
 // The larger values of two words, element by element, NaN where either is.
@@ -150,6 +155,11 @@ __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b) {
     else if (std::is_same<T, __nv_bfloat16>::value) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
     else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
     return y;
+}
+// Whether a word of fp16, the smallest elements met, has a -inf.
+template <typename T>
+__device__ __forceinline__ bool has_minus_inf(uint32_t low) {
+    return std::is_same<T, __half>::value && ((low & 0xFFFFu) == 0xFC00u || low >> 16 == 0xFC00u);
 }
 template <typename T>
 __device__ __forceinline__ float word_top(uint32_t w) {
@@ -280,15 +290,15 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
 #pragma unroll 4
         for (int j = tid; j < r.A; j += threads)
             if (legal(bits, j)) {
-                const float d = to_f32(z[j]) - q.m, e = ex2(d * kLog2e), dl = fmaxf(d, kLow), y = second(j);
+                const float d = to_f32(z[j]) - q.m, e = ex2(d * kLog2e), dl = fmaxf(d, kLow<T>), y = second(j);
                 q.s += e;
                 q.t = fmaf(e, dl, q.t);
                 if (KIND == kSearch) { q.a = fmaf(y, dl, q.a); q.b += y; }
-                if (KIND == kClippedRef) { q.a = fmaf(e, dl - fmaxf(y - q.c, kLow), q.a); q.b += ex2((y - q.c) * kLog2e); }
+                if (KIND == kClippedRef) { q.a = fmaf(e, dl - fmaxf(y - q.c, kLow<T>), q.a); q.b += ex2((y - q.c) * kLog2e); }
             }
     q.s = join(q.s, false); q.t = join(q.t, false);
     if (KIND != kClipped) { q.a = join(q.a, false); q.b = join(q.b, false); }
-    if (q.za != -kInf) q.za = max_nan(q.za, q.m + kLow);
+    if (q.za != -kInf) q.za = max_nan(q.za, q.m + kLow<T>);
     RowGrad g;
     RowOut out;
     live = row_result<KIND>(r, q, w, KIND == kSearch ? 0.f : r.old_logp[row], KIND == kSearch ? 0.f : r.advantage[row], &g, &out) && live;
@@ -297,9 +307,9 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
     for (int j = tid; j < r.A; j += threads) {
         float o = 0.f;
         if (live && legal(bits, j)) {
-            const float d = to_f32(z[j]) - g.M, dl = fmaxf(d, kLow), y = second(j);
+            const float d = to_f32(z[j]) - g.M, dl = fmaxf(d, kLow<T>), y = second(j);
             o = fmaf(g.kz, dl, g.k0);
-            if (KIND == kClippedRef) o = fmaf(g.kd, dl - fmaxf(y - g.C, kLow), o);
+            if (KIND == kClippedRef) o = fmaf(g.kd, dl - fmaxf(y - g.C, kLow<T>), o);
             o *= ex2(fmaf(d, kLog2e, g.lp));
             if (KIND == kSearch) o = fmaf(-g.kt, y, o);
             else if (j == act) o += g.ka;
@@ -389,6 +399,10 @@ struct Part {
     bool first_out, last_out;
 };
 
+// What the first pass finds in its vectors: the largest words of both matrices; fp16: the smallest of either.
+struct Tops { uint32_t z, x, low; };
+__device__ __forceinline__ void word_min(uint32_t& low, uint32_t w) { asm("min.f16x2 %0, %0, %1;" : "+r"(low) : "r"(w)); }
+
 // The words of vector v of a part.
 template <typename T, int KIND>
 struct Vec {
@@ -433,15 +447,17 @@ struct Vec {
 #pragma unroll
         for (int i = 0; i < XW; ++i) x[i] = __float_as_uint((float)(int)x[i]);
     }
-    // Not below the lowest value; the largest words.
-    __device__ __forceinline__ void raise(uint32_t* top_z, uint32_t* top_x) {
+    // The largest words; not below the lowest value, or, in fp16, the smallest words too.
+    __device__ __forceinline__ void raise(Tops& t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            z[i] = word_max<T>(z[i], Lowest<T>::kWord);
-            *top_z = word_max<T>(*top_z, z[i]);
+            if (std::is_same<T, __half>::value) word_min(t.low, z[i]);
+            else z[i] = word_max<T>(z[i], Lowest<T>::kWord);
+            t.z = word_max<T>(t.z, z[i]);
             if (KIND == kClippedRef) {
-                x[i % XW] = word_max<T>(x[i % XW], Lowest<T>::kWord);
-                *top_x = word_max<T>(*top_x, x[i % XW]);
+                if (std::is_same<T, __half>::value) word_min(t.low, x[i % XW]);
+                else x[i % XW] = word_max<T>(x[i % XW], Lowest<T>::kWord);
+                t.x = word_max<T>(t.x, x[i % XW]);
             }
         }
     }
@@ -491,7 +507,7 @@ __device__ __noinline__ void fetch_vector(const PolicyRows& r, long long row, co
 // 0), visit counts become fp32.  Returns whether any action met was legal.
 // SHORT: rows of a few vectors a thread take their outer vectors along in the loop; the others' loops are free of them.
 template <typename T, int KIND, bool ALIKE, int U, bool SHORT>
-__device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, const Part& p, int tid, int stride, uint32_t* top_z, uint32_t* top_x) {
+__device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, const Part& p, int tid, int stride, Tops& tops) {
     constexpr int V = 16 / sizeof(T);
     uint32_t any = r.bits ? 0u : ~0u;
     using W = Vec<T, KIND>;
@@ -513,7 +529,7 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
                 w.keep(on);
             }
             if (KIND == kSearch && r.visits) w.counts_to_f32();
-            w.raise(top_z, top_x);
+            w.raise(tops);
             w.store_z(p, v);
             if (KIND == kClippedRef || (KIND == kSearch && (change || r.visits))) w.store_x(p, v);
         }
@@ -534,7 +550,7 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
                 if (r.visits) w.counts_to_f32();
                 w.store_x(p, v);
             }
-            w.raise(top_z, top_x);
+            w.raise(tops);
             w.store_z(p, v);
             if (KIND == kClippedRef) w.store_x(p, v);
         }
@@ -545,7 +561,7 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
             w.load_x(p, v);
             w.counts_to_f32();
             w.store_x(p, v);
-            w.raise(top_z, top_x);
+            w.raise(tops);
             w.store_z(p, v);
         }
     } else {
@@ -558,7 +574,7 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                w[u].raise(top_z, top_x);
+                w[u].raise(tops);
                 w[u].store_z(p, v + u * stride);
                 if (KIND == kClippedRef) w[u].store_x(p, v + u * stride);
             }
@@ -567,7 +583,7 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
             W w;
             w.load_z(p, v);
             if (KIND == kClippedRef) w.load_x(p, v);
-            w.raise(top_z, top_x);
+            w.raise(tops);
             w.store_z(p, v);
             if (KIND == kClippedRef) w.store_x(p, v);
         }
@@ -584,7 +600,7 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
         any |= on & ((1u << V) - 1);
         w.keep(on);
         if (KIND == kSearch && r.visits) w.counts_to_f32();
-        w.raise(top_z, top_x);
+        w.raise(tops);
         w.store_z(p, e);
         w.store_x(p, e);
     }
@@ -592,7 +608,7 @@ __device__ __forceinline__ bool pass_max(const PolicyRows& r, long long row, con
 }
 
 // Second pass: the sums relative to q.m and q.c.
-template <typename T, int KIND, int U>
+template <typename T, int KIND, int U, bool FLOOR>
 __device__ __forceinline__ void pass_sums(const Part& p, int tid, int stride, Sums& q) {
     constexpr int V = 16 / sizeof(T);
     using W = Vec<T, KIND>;
@@ -601,7 +617,7 @@ __device__ __forceinline__ void pass_sums(const Part& p, int tid, int stride, Su
     auto add = [&](const W& w) {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
-            const f32x2 d = elements_less<T>(w.z, i, M, q.m), e = ex2_2(mul2(d, L));
+            const f32x2 d = elements_less<T, FLOOR>(w.z, i, M, q.m), e = ex2_2(mul2(d, L));
             s = add2(s, e);
             t = fma2(e, d, t);
             if (KIND == kSearch) {
@@ -610,7 +626,7 @@ __device__ __forceinline__ void pass_sums(const Part& p, int tid, int stride, Su
                 b = add2(b, y);
             }
             if (KIND == kClippedRef) {
-                const f32x2 c = elements_less<T>(w.x, i, C, q.c);
+                const f32x2 c = elements_less<T, FLOOR>(w.x, i, C, q.c);
                 b = add2(b, ex2_2(mul2(c, L)));
                 a = fma2(e, fma2(c, minus, d), a);
             }
@@ -635,7 +651,7 @@ __device__ __forceinline__ void pass_sums(const Part& p, int tid, int stride, Su
 
 // Third pass: the gradient (0 where the row is not live), to `grad` (the row's element 0 stands at grad + head), or into
 // the slot where stores of vectors are not possible.
-template <typename T, int KIND, bool ALIKE, int U, bool SHORT>
+template <typename T, int KIND, bool ALIKE, int U, bool SHORT, bool FLOOR>
 __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, int tid, int stride, bool live, const RowGrad& g, int act_e, T* grad) {
     constexpr int V = 16 / sizeof(T);
     using W = Vec<T, KIND>;
@@ -650,9 +666,9 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
     const bool act_mine = KIND != kSearch && live && act_e >= p.v0 * V && act_e < p.v1 * V && act_at / V % stride == tid;
     float act_grad = 0.f;
     if (act_mine) {
-        const float d = to_f32(in_shared<const T>(p.zs)[act_at]) - g.M;
+        const float d = max_nan(to_f32(in_shared<const T>(p.zs)[act_at]) - g.M, kLow<T>);
         float y = fmaf(kzd, d, g.k0);
-        if (KIND == kClippedRef) y = fmaf(-g.kd, to_f32(in_shared<const T>(p.xs)[act_at]) - g.C, y);
+        if (KIND == kClippedRef) y = fmaf(-g.kd, max_nan(to_f32(in_shared<const T>(p.xs)[act_at]) - g.C, kLow<T>), y);
         act_grad = fmaf(y, ex2(fmaf(d, kLog2e, g.lp)), g.ka);
     }
     auto put_act = [&] {
@@ -665,9 +681,9 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
         float o[V];
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
-            const f32x2 d = elements_less<T>(w.z, i, M, g.M), pr = ex2_2(fma2(d, L, lp));
+            const f32x2 d = elements_less<T, FLOOR>(w.z, i, M, g.M), pr = ex2_2(fma2(d, L, lp));
             f32x2 y = fma2(kz, d, k0);
-            if (KIND == kClippedRef) y = fma2(kd, elements_less<T>(w.x, i, C, g.C), y);
+            if (KIND == kClippedRef) y = fma2(kd, elements_less<T, FLOOR>(w.x, i, C, g.C), y);
             y = mul2(y, pr);
             if (KIND == kSearch) y = fma2(kt, elements<float>(w.x, i), y);
             halves(y, o[2 * i], o[2 * i + 1]);
@@ -757,6 +773,10 @@ __device__ __forceinline__ void pass_grad(const PolicyRows& r, const Part& p, in
     }
     put_act();
 }
+
+// The action's logit from element `at` of the slot; -inf as a difference of it counts.
+template <typename T>
+__device__ __forceinline__ float action_logit(const Part& p, int at) { return max_nan(to_f32(in_shared<const T>(p.zs)[at]), kLow<T>); }
 
 // Without vectors: what a team holds of a row, element by element, into its slot and back.
 template <typename T, int KIND>
@@ -868,23 +888,27 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         const int act = KIND == kSearch ? -1 : __float_as_int(scalars.w);
         const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;       // the action's element of the row
         bool live = is && w != 0.f, apart = false;
-        uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
-        const bool some = live && pass_max<T, KIND, ALIKE, U, (LANES < 32)>(r, row, p, tid, LANES, &top_z, &top_x);
+        Tops tops{Lowest<T>::kWord, Lowest<T>::kWord, Lowest<T>::kWord};
+        const bool some = live && pass_max<T, KIND, ALIKE, U, (LANES < 32)>(r, row, p, tid, LANES, tops);
+        const bool floored = std::is_same<T, __half>::value && __any_sync(~0u, has_minus_inf<T>(tops.low));
         // rows without a legal action are left out
         if (LANES == 32) live = __any_sync(~0u, some);
         else live = (__ballot_sync(~0u, some) >> (lane & ~(LANES - 1))) & ((1u << (LANES & 31)) - 1);
         Sums q;
-        q.m = team_max_nan<LANES>(word_top<T>(top_z));
-        q.c = KIND == kClippedRef ? team_max_nan<LANES>(word_top<T>(top_x)) : 0.f;
+        q.m = team_max_nan<LANES>(word_top<T>(tops.z));
+        q.c = KIND == kClippedRef ? team_max_nan<LANES>(word_top<T>(tops.x)) : 0.f;
         __syncwarp();
         q.za = -kInf;
-        if (KIND != kSearch && live && act_e >= 0 && (!r.bits || (load_word(p.ms + 4 * (act >> 5)) >> (act & 31)) & 1u)) q.za = to_f32(in_shared<const T>(p.zs)[act_e]);
+        if (KIND != kSearch && live && act_e >= 0 && (!r.bits || (load_word(p.ms + 4 * (act >> 5)) >> (act & 31)) & 1u)) q.za = action_logit<T>(p, act_e);
         if (live && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2))) apart = true;
         for (uint32_t m = __ballot_sync(~0u, apart && tid == 0); m; m &= m - 1)
             careful_row<T, KIND>(r, __shfl_sync(~0u, row, __ffs(m) - 1));
         live = live && !apart;
         q.s = q.t = q.a = q.b = 0.f;
-        if (live) pass_sums<T, KIND, U>(p, tid, LANES, q);
+        if (live) {
+            if (floored) pass_sums<T, KIND, U, true>(p, tid, LANES, q);
+            else pass_sums<T, KIND, U, false>(p, tid, LANES, q);
+        }
         q.s = team_sum<LANES>(q.s);
         q.t = team_sum<LANES>(q.t);
         if (KIND != kClipped) { q.a = team_sum<LANES>(q.a); q.b = team_sum<LANES>(q.b); }
@@ -894,7 +918,10 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         if (tid == 0 && is && !apart) put_out(r, row, live, out);
         T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
         __syncwarp();                            // the gradient may take the place of the action's logit
-        if (!apart) pass_grad<T, KIND, ALIKE, U, (LANES < 32)>(r, p, tid, LANES, live, g, act_e, grad);
+        if (!apart) {
+            if (floored) pass_grad<T, KIND, ALIKE, U, (LANES < 32), true>(r, p, tid, LANES, live, g, act_e, grad);
+            else pass_grad<T, KIND, ALIKE, U, (LANES < 32), false>(r, p, tid, LANES, live, g, act_e, grad);
+        }
         if (ALIKE) {
             // the slot's next copy comes behind what was read and written here
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1021,24 +1048,26 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
         }
         const int act = KIND == kSearch ? -1 : __float_as_int(scalars.w);
         const int act_e = (unsigned)act < (unsigned)r.A ? act + p.head : -1;       // the action's element of the row
-        bool live = w != 0.f, apart = false;
+        bool live = w != 0.f, apart = false, floored = false;
         RowGrad g;
         RowOut out;
         if (live) {                              // the same in the whole team
-            uint32_t top_z = Lowest<T>::kWord, top_x = Lowest<T>::kWord;
-            const bool some = __any_sync(~0u, pass_max<T, KIND, ALIKE, U, false>(r, row, p, threadIdx.x, threads, &top_z, &top_x));
-            const float top = warp_max_nan(word_top<T>(top_z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(top_x)) : 0.f;
+            Tops tops{Lowest<T>::kWord, Lowest<T>::kWord, Lowest<T>::kWord};
+            const bool some = __any_sync(~0u, pass_max<T, KIND, ALIKE, U, false>(r, row, p, threadIdx.x, threads, tops));
+            floored = std::is_same<T, __half>::value && __any_sync(~0u, has_minus_inf<T>(tops.low));
+            const float top = warp_max_nan(word_top<T>(tops.z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(tops.x)) : 0.f;
             __syncwarp();
             // The action's logit, by the warp that has its vector and ahead of the meeting: behind it the others may find the
             // gradient in its place.
             const int act_at = KIND != kSearch && act_e >= v0 * V && act_e < p.v1 * V && (!r.bits || (load_word(p.ms + 4 * ((act >> 5) - p.mask_first)) >> (act & 31)) & 1u)
                                    ? act_e - v0 * V : -1;
             float za = -kInf;
-            if (KIND != kSearch && act_at >= 0 && act_at / V % threads / 32 == warp) za = to_f32(in_shared<const T>(p.zs)[act_at]);
+            if (KIND != kSearch && act_at >= 0 && act_at / V % threads / 32 == warp) za = action_logit<T>(p, act_at);
             Sums q;
             q.m = base_of<T>(top);
             q.c = KIND == kClippedRef ? base_of<T>(top_ref) : 0.f;
-            pass_sums<T, KIND, U>(p, threadIdx.x, threads, q);
+            if (floored) pass_sums<T, KIND, U, true>(p, threadIdx.x, threads, q);
+            else pass_sums<T, KIND, U, false>(p, threadIdx.x, threads, q);
             const float sum = four_sums(q.s, q.t, q.a, q.b);
             float (*all)[8] = part[turn];
             turn ^= 1;
@@ -1065,7 +1094,10 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
         }
         if (threadIdx.x == 0 && cta == 0 && !apart) put_out(r, row, live, out);
         T* const grad = (T*)r.grad + row * r.g_pitch - p.head;
-        if (!apart) pass_grad<T, KIND, ALIKE, U, false>(r, p, threadIdx.x, threads, live, g, act_e, grad);
+        if (!apart) {
+            if (floored) pass_grad<T, KIND, ALIKE, U, false, true>(r, p, threadIdx.x, threads, live, g, act_e, grad);
+            else pass_grad<T, KIND, ALIKE, U, false, false>(r, p, threadIdx.x, threads, live, g, act_e, grad);
+        }
         if (ALIKE) {
             // the next copy comes behind what was read and written here
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

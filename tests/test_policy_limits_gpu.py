@@ -1,8 +1,9 @@
-"""Policy losses at the ends of what the header allows: reference policies without any probability."""
+"""Policy losses at the ends of what the header allows: reference policies without any probability, logits of -inf where
+something is asked of them."""
 import numpy as np
 import pytest
 
-from test_policy_loss_gpu import TYPES, dtype_of, half_step, pack, ref_clipped, relative_bound
+from test_policy_loss_gpu import TYPES, dtype_of, half_step, pack, ref_clipped, ref_search, relative_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -14,6 +15,11 @@ INF = float("inf")
 def api(lib):
     from omoknuni_small_b200 import capi
     return capi
+
+
+def floor_of(dt):
+    """What a difference of logits of -inf counts as."""
+    return -1.5703125 * 2.0 ** 99 if dt == "bf16" else -1e30
 
 
 def cuda(a):
@@ -64,3 +70,100 @@ def test_reference_without_any_probability(api, dt, A, many):
             assert (np.abs(stats[rows] - rs)[:, keep] <= (E * (1 + np.abs(rs)))[:, keep]).all()
             if k == kappa or not kappa:
                 assert (np.abs(loss[rows] - rl) <= E * (np.abs(rl) + lterm + w[rows])).all()
+
+
+@pytest.mark.parametrize("unlike", [False, True], ids=["alike", "unlike"])
+@pytest.mark.parametrize("A", LENGTHS)
+@pytest.mark.parametrize("dt", TYPES)
+def test_targets_at_logits_of_minus_infinity(api, dt, A, unlike):
+    """A legal logit of -inf that the target wants, in the same measure whatever the type and the length; rows that want none
+    of theirs are as if those were not legal."""
+    import torch
+    n = 40
+    T = dtype_of(dt)
+    rng = np.random.default_rng(A + 1)
+    z = torch.from_numpy(rng.normal(0, 2, (n, A)).astype(np.float32)).to(T)
+    t = rng.gamma(1.0, 1.0, (n, A)).astype(np.float32)
+    gone = rng.random((n, A)) < 0.2
+    gone[:, 0] = False
+    gone[::2, A - 1] = gone[1::4, A // 2] = True
+    z64 = z.double().numpy()
+    t[gone] = 0
+    wanted = np.arange(n) % 2 == 0
+    share = np.float32(0.01)
+    t[wanted, A - 1] = t[wanted].sum(1) * share / (1 - share)
+    zc = z.clone()
+    zc[torch.from_numpy(gone)] = -INF
+    zd = zc.cuda()
+    if unlike:
+        zd = torch.nn.functional.pad(zd, (0, 3))[:, :A]
+    loss, grad, stats = [x.double().cpu().numpy() for x in api.policy_loss_search(zd, cuda(t), entropy_coef=0.05)]
+    rl, rg, rs, terms = ref_search(z64, ~gone, np.where(gone, 0, t).astype(float), np.ones(n), 0.05)
+    # the reference above knows nothing of what is gone: its pi is of the rest
+    t64 = t.astype(float)
+    pi_all = t64 / t64.sum(1, keepdims=True)
+    want_g = rg + np.where(gone, 0, t64) / np.where(gone, 0, t64).sum(1, keepdims=True) - pi_all
+    reach = 2 * np.abs(z64).max() + 1
+    D = relative_bound(A, reach)
+    half, least = half_step(T)
+    assert (np.abs(grad - want_g) <= 4 * D * (terms + pi_all) + half * np.abs(want_g) + least).all()
+    missing = np.where(gone, pi_all, 0).sum(1)
+    ce = rs[:, 0] * (1 - missing) + missing * -floor_of(dt)
+    # a rounding for each of the products and sums of 1e30, besides those of the ordinary ones
+    assert (np.abs(stats[:, 0] - ce) <= 4 * D * (1 + reach + ce)).all()
+    assert (np.abs(stats[:, 1] - rs[:, 1]) <= 4 * D * (1 + reach + rs[:, 1])).all()
+    assert (np.abs(loss - (ce - 0.05 * rs[:, 1])) <= 4 * D * (1 + reach + ce) * 1.05).all()
+
+
+@pytest.mark.parametrize("A", LENGTHS)
+@pytest.mark.parametrize("dt", TYPES)
+def test_actions_the_reference_excludes(api, dt, A):
+    """KL counts an action that q excludes as -1e30, whatever the type and the length; an action whose own logit is -inf has
+    the ratio 0 and no gradient."""
+    import torch
+    n = 24
+    T = dtype_of(dt)
+    rng = np.random.default_rng(A + 2)
+    z = torch.from_numpy(rng.normal(0, 2, (n, A)).astype(np.float32)).to(T)
+    zr = torch.from_numpy(rng.normal(0, 2, (n, A)).astype(np.float32)).to(T)
+    at = A // 3
+    zr[::3, at] = -INF                           # excluded by q
+    z[1::3, at] = zr[1::3, at] = -INF            # by both: nothing to count
+    act = np.full(n, at, np.int32)
+    act[::3] = 0
+    z64, r64 = z.double().numpy(), zr.double().numpy()
+    legal = np.ones((n, A), bool)
+    legal[1::3, at] = False                      # for the reference result: p is 0 there
+    low = floor_of(dt)
+    logp = z64 - np.where(legal, z64, -INF).max(1, keepdims=True)
+    d = np.where(legal, logp, low)
+    e = np.where(legal, np.exp(d), 0)
+    p = e / e.sum(1, keepdims=True)
+    lp = np.where(legal, d - np.log(e.sum(1, keepdims=True)), 0)
+    dr = r64 - np.where(np.isfinite(r64), r64, -INF).max(1, keepdims=True)
+    dr = np.where(np.isfinite(dr), dr, low)
+    x = np.where(legal, lp - (dr - np.log(np.exp(dr).sum(1, keepdims=True))), 0)
+    kl = (p * x).sum(1)
+    kappa, w = 0.25, rng.uniform(0.5, 2, n).astype(np.float32)
+    loss, grad, stats = api.policy_loss_clipped(z.cuda(), cuda(act), cuda(np.zeros(n, np.float32)), cuda(np.zeros(n, np.float32)), None, zr.cuda(),
+                                                cuda(w), kl_coef=kappa)
+    loss, stats = loss.double().cpu().numpy(), stats.double().cpu().numpy()
+    reach = 2 * max(np.abs(z64[legal]).max(), np.abs(r64[np.isfinite(r64)]).max()) + 1
+    D = relative_bound(A, reach)
+    size = (p * np.abs(x)).sum(1)
+    assert (np.abs(stats[:, 2] - kl) <= 4 * D * (1 + reach + size)).all()
+    assert (np.abs(loss - w * kappa * kl) <= 4 * D * w * (1 + reach + size)).all()
+    gone = np.arange(n) % 3 == 1
+    assert (stats[gone, 1] == 0).all() and (np.abs(stats[gone, 0] / low - 1) <= 2.0 ** -20).all()
+    # in fp32: what is beyond the gradient's type becomes infinite in it
+    want = w[:, None] * kappa * p * (x - kl[:, None])
+    tol = 4 * D * w[:, None] * kappa * p * (np.abs(x) + size[:, None] + 1)
+    top = float(torch.finfo(T).max)
+    got = grad.double().cpu().numpy()
+    half, least = half_step(T)
+    big = np.abs(want) > top
+    sure = np.abs(want) - tol > top * (1 + half)
+    assert (got[sure] == np.sign(want[sure]) * INF).all()
+    fine = ~big & (np.abs(want) + tol < top)
+    assert (np.abs(got - want)[fine] <= (tol + half * np.abs(want) + least)[fine]).all()
+    assert (got[gone, at] == 0).all()
