@@ -250,6 +250,12 @@ __device__ __forceinline__ void put_out(const PolicyRows& r, long long row, bool
     if (r.stats) r.stats[row] = live ? o.stats : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
+// Targets whose sum T, times differences down to -1e30 and as a divisor of a row's weight, stays well within fp32: a row with
+// others is scaled by a power of two, by careful_row.  NaN is taken as it is.
+__device__ __forceinline__ bool target_fits(float T) { return !(T > 0x1p27f || (T < 0x1p-60f && T != 0.f)); }
+// Largest logits beyond the floor's size: differences from them would be below it where the other passes do not look.
+template <typename T> __device__ __forceinline__ bool too_high(float m) { return !std::is_same<T, __half>::value && m > -kLow<T>; }
+
 __device__ __forceinline__ bool legal(const uint32_t* bits, int j) { return !bits || (bits[j >> 5] >> (j & 31)) & 1u; }
 __device__ __forceinline__ float target_f32(uint32_t raw, int visits) { return visits ? (float)(int)raw : __uint_as_float(raw); }
 
@@ -298,10 +304,25 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
             }
     q.s = join(q.s, false); q.t = join(q.t, false);
     if (KIND != kClipped) { q.a = join(q.a, false); q.b = join(q.b, false); }
+    const float total = q.b;
+    float unit = 1.f;                            // of the targets
+    if (KIND == kSearch && !target_fits(total)) {
+        unit = __uint_as_float((254u - min(max((__float_as_uint(total) & 0x7FFFFFFFu) >> 23, 1u), 253u)) << 23);
+        q.a = q.b = 0.f;
+        if (live)
+            for (int j = tid; j < r.A; j += threads)
+                if (legal(bits, j)) {
+                    const float y = second(j) * unit;
+                    q.a = fmaf(y, fmaxf(to_f32(z[j]) - q.m, kLow<T>), q.a);
+                    q.b += y;
+                }
+        q.a = join(q.a, false); q.b = join(q.b, false);
+    }
     if (q.za != -kInf) q.za = max_nan(q.za, q.m + kLow<T>);
     RowGrad g;
     RowOut out;
     live = row_result<KIND>(r, q, w, KIND == kSearch ? 0.f : r.old_logp[row], KIND == kSearch ? 0.f : r.advantage[row], &g, &out) && live;
+    if (KIND == kSearch) out.stats.z = total;
     if (tid == 0) put_out(r, row, live, out);
 #pragma unroll 4
     for (int j = tid; j < r.A; j += threads) {
@@ -311,14 +332,15 @@ __device__ __forceinline__ void plain_row(const PolicyRows& r, long long row, in
             o = fmaf(g.kz, dl, g.k0);
             if (KIND == kClippedRef) o = fmaf(g.kd, dl - fmaxf(y - g.C, kLow<T>), o);
             o *= ex2(fmaf(d, kLog2e, g.lp));
-            if (KIND == kSearch) o = fmaf(-g.kt, y, o);
+            if (KIND == kSearch) o = fmaf(-g.kt, y * unit, o);
             else if (j == act) o += g.ka;
         }
         grad[j] = from_f32<T>(o);
     }
 }
 
-// Rows without an ordinary logit - all of them at a type's lowest value or -inf - by one warp.
+// Rows without an ordinary logit (all of them at a type's lowest value or -inf), with one beyond 1e30 or with targets of
+// an extreme scale, by one warp.
 template <typename T, int KIND>
 __device__ __noinline__ void careful_row(const PolicyRows& r, long long row) {
     plain_row<T, KIND>(r, row, threadIdx.x % 32, 32, [](float v, bool is_max) { return is_max ? warp_max_nan(v) : team_sum(v); });
@@ -900,18 +922,17 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         __syncwarp();
         q.za = -kInf;
         if (KIND != kSearch && live && act_e >= 0 && (!r.bits || (load_word(p.ms + 4 * (act >> 5)) >> (act & 31)) & 1u)) q.za = action_logit<T>(p, act_e);
-        if (live && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2))) apart = true;
-        for (uint32_t m = __ballot_sync(~0u, apart && tid == 0); m; m &= m - 1)
-            careful_row<T, KIND>(r, __shfl_sync(~0u, row, __ffs(m) - 1));
-        live = live && !apart;
+        apart = live && (q.m < Lowest<T>::kValue / 2 || too_high<T>(q.m) || (KIND == kClippedRef && (q.c < Lowest<T>::kValue / 2 || too_high<T>(q.c))));
         q.s = q.t = q.a = q.b = 0.f;
-        if (live) {
+        if (live && !apart) {
             if (floored) pass_sums<T, KIND, U, true>(p, tid, LANES, q);
             else pass_sums<T, KIND, U, false>(p, tid, LANES, q);
         }
         q.s = team_sum<LANES>(q.s);
         q.t = team_sum<LANES>(q.t);
         if (KIND != kClipped) { q.a = team_sum<LANES>(q.a); q.b = team_sum<LANES>(q.b); }
+        if (KIND == kSearch && live && !target_fits(q.b)) apart = true;
+        live = live && !apart;
         RowGrad g;
         RowOut out;
         live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && live;
@@ -922,6 +943,8 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
             if (floored) pass_grad<T, KIND, ALIKE, U, (LANES < 32), true>(r, p, tid, LANES, live, g, act_e, grad);
             else pass_grad<T, KIND, ALIKE, U, (LANES < 32), false>(r, p, tid, LANES, live, g, act_e, grad);
         }
+        for (uint32_t m = __ballot_sync(~0u, apart && tid == 0); m; m &= m - 1)
+            careful_row<T, KIND>(r, __shfl_sync(~0u, row, __ffs(m) - 1));
         if (ALIKE) {
             // the slot's next copy comes behind what was read and written here
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1088,7 +1111,8 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             }
             q = join_entries<T, KIND>(all, (int)ctas * warps);
             const bool legal_one = __any_sync(~0u, lane < (int)ctas * warps && all[lane][7] != 0.f);      // else the row is left out
-            apart = legal_one && (q.m < Lowest<T>::kValue / 2 || (KIND == kClippedRef && q.c < Lowest<T>::kValue / 2));
+            apart = legal_one && (q.m < Lowest<T>::kValue / 2 || too_high<T>(q.m) || (KIND == kSearch && !target_fits(q.b)) ||
+                                  (KIND == kClippedRef && (q.c < Lowest<T>::kValue / 2 || too_high<T>(q.c))));
             live = row_result<KIND>(r, q, w, scalars.y, scalars.z, &g, &out) && legal_one;
             if (apart && warp == 0 && cta == 0) careful_row<T, KIND>(r, row);
         }

@@ -1,5 +1,7 @@
 """Policy losses at the ends of what the header allows: reference policies without any probability, logits of -inf where
-something is asked of them."""
+something is asked of them, very large logits, targets of any scale."""
+import math
+
 import numpy as np
 import pytest
 
@@ -167,3 +169,72 @@ def test_actions_the_reference_excludes(api, dt, A):
     fine = ~big & (np.abs(want) + tol < top)
     assert (np.abs(got - want)[fine] <= (tol + half * np.abs(want) + least)[fine]).all()
     assert (got[gone, at] == 0).all()
+
+
+@pytest.mark.parametrize("A", LENGTHS)
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("total", [1e-37, 1e-30, 1e-15, 1e7, 1e9, 1e20, 1e30, 8e37])
+def test_targets_of_any_scale(api, dt, A, total):
+    """Loss and gradient do not depend on the scale of the targets, with logits far apart and the weight of a loss scale."""
+    import torch
+    n = 10
+    T = dtype_of(dt)
+    rng = np.random.default_rng(A + 3)
+    z = torch.from_numpy(rng.normal(0, 8, (n, A)).astype(np.float32)).to(T)
+    t = rng.gamma(0.5, 1.0, (n, A))
+    t = (t / t.sum(1, keepdims=True) * total).astype(np.float32)
+    t[3] = 0
+    legal = rng.random((n, A)) < 0.8
+    legal[:, 1] = True
+    w = np.full(n, 1024.0, np.float32)
+    z64 = z.double().numpy()
+    loss, grad, stats = [x.double().cpu().numpy() for x in api.policy_loss_search(z.cuda(), cuda(t), pack(legal), cuda(w), entropy_coef=0.05)]
+    rl, rg, rs, terms = ref_search(z64, legal, t.astype(float), w.astype(float), 0.05)
+    reach = 2 * np.abs(z64).max() + 1
+    D = relative_bound(A, reach)
+    half, least = half_step(T)
+    top = float(torch.finfo(T).max)
+    assert np.abs(rg).max() < top
+    assert (np.abs(grad - rg) <= 4 * D * terms + half * np.abs(rg) + least).all()
+    assert (np.abs(stats - rs) <= 4 * D * np.stack([1 + reach + rs[:, 0], 1 + reach + rs[:, 1], rs[:, 2], 1 + reach + np.abs(rs[:, 3])], 1)).all()
+    assert (np.abs(loss - rl) <= 4 * D * (np.abs(rl) + w * 1.05 * (1 + reach))).all()
+
+
+@pytest.mark.parametrize("A", LENGTHS)
+def test_visit_counts_beyond_32_bits_in_sum(api, A):
+    """The largest counts, some of them at logits of -inf: 6e9 visits of which a third are at -1e30."""
+    import torch
+    z = np.zeros((3, A), np.float32)
+    z[:, 5] = -INF
+    z[1] = -INF
+    z[1, 2] = 0
+    t = np.zeros((3, A), np.int32)
+    t[0, [2, 4, 5]] = t[1, [2, 4, 5]] = 2000000000
+    t[2, 2] = 2147483647
+    loss, grad, stats = [x.double().cpu().numpy() for x in api.policy_loss_search(cuda(z), cuda(t))]
+    D = relative_bound(A, 1)
+    assert abs(stats[0, 0] - 1e30 / 3) <= 4 * D * 1e30 and abs(stats[1, 0] - 2e30 / 3) <= 4 * D * 1e30
+    assert abs(stats[2, 0] - math.log(A - 1)) <= 4 * D * (1 + math.log(A))
+    assert np.allclose(stats[:, 2], [6e9, 6e9, 2147483647.0], rtol=2.0 ** -22) and np.isfinite(loss).all()
+    assert abs(grad[1, 4] + 1 / 3) <= 4 * D and abs(grad[1, 2] - 2 / 3) <= 4 * D and abs(grad[0, 5] + 1 / 3) <= 4 * D
+
+
+@pytest.mark.parametrize("A", LENGTHS)
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_very_large_logits(api, dt, A):
+    """One logit of 1e36 among ordinary ones: the policy is that action, the others count as -1e30."""
+    import torch
+    T = dtype_of(dt)
+    z = torch.zeros((2, A), dtype=T)
+    z[:, 3] = 1e36
+    z[1] *= -1                                   # one logit of -1e36 among zeros
+    t = np.full((2, A), 800, np.int32)
+    loss, grad, stats = [x.double().cpu().numpy() for x in api.policy_loss_search(z.cuda(), cuda(t), entropy_coef=0.05)]
+    D, low = relative_bound(A, 1), floor_of(dt)
+    half = half_step(T)[0]
+    ce = np.array([(A - 1) / A * -low, -low / A])
+    # of the second row's, in the order of 1e30, the logarithm is lost
+    assert (np.abs(stats[:, 0] - ce) <= (4 * D + 2.0 ** -20) * ce).all()
+    assert stats[0, 1] == 0 and abs(stats[1, 1] - math.log(A - 1)) <= 4 * D * (1 + math.log(A))
+    assert abs(grad[0, 3] - (A - 1) / A) <= 4 * D + half and (np.abs(grad[0, 4:] + 1 / A) <= (4 * D + half) / A).all()
+    assert abs(grad[1, 3] + 1 / A) <= (4 * D + half) / A
