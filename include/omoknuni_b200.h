@@ -678,6 +678,11 @@ int ob200_copy_to_host(void* dst_host, const void* src_device, int64_t bytes);
  *  and its optimiser step from PyTorch's elementary operations; these are the
  *  same kind of step as single launches over caller-owned DEVICE memory of the
  *  current device, asynchronous on `stream`, capturable, without allocation.
+ *  A kernel whose bounded wait for a copy runs out raises the device's error word
+ *  (code 4, ob200_device_error_code; the next host-buffer call or search on the
+ *  device reports it too) and leaves NaN as loss, statistics and gradient of the
+ *  rows it did not finish, so that ob200_launch_grad_norm gives a factor with which
+ *  ob200_launch_adamw leaves the step out.
  *  Sums, softmax statistics and norms are held in 32 bits or more; results do
  *  not depend on the order in which CTAs run.
  * ------------------------------------------------------------------------- */
@@ -746,6 +751,9 @@ int ob200_launch_policy_loss_clipped(const ob200_policy_rows* rows, const int32_
                                      const float* advantage, const void* ref_logits, int64_t ref_pitch,
                                      float clip_low, float clip_high, float kl_coef, float entropy_coef,
                                      ob200_stream stream);
+/* Test hook: with give_up != 0 the waits of the policy losses' kernels run out at
+ * once in every later call of the process, with 0 they wait again. */
+void ob200_debug_policy_waits(int32_t give_up);
 
 /* One trained tensor.  `tensors` arguments below are HOST arrays, read before the
  * call returns; the memory they name belongs to the device.  Pointers need the

@@ -18,7 +18,7 @@ RULES_FREESTYLE, RULES_OMOK, RULES_RENJU = 0, 1, 2
 DTYPE_BF16, DTYPE_F16 = 0, 1     # storage type of board tensors and packed tower weights
 DTYPE_F32 = 2                    # policy rows, gradients and weights of the training operators
 TARGET_VISITS, TARGET_PROBS = 0, 1
-ERR_INVALID = 1
+ERR_INVALID, ERR_TIMEOUT = 1, 6
 
 
 class Error(RuntimeError):
@@ -174,6 +174,7 @@ SIGNATURES = {
     "ob200_launch_policy_loss_search": (C.c_int, [C.POINTER(PolicyRows), C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_void_p]),
     "ob200_launch_policy_loss_clipped": (C.c_int, [C.POINTER(PolicyRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                                    C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float, C.c_void_p]),
+    "ob200_debug_policy_waits": (None, [C.c_int32]),
     "ob200_grad_norm_workspace_bytes": (C.c_int64, []),
     "ob200_launch_grad_norm": (C.c_int, [C.POINTER(TrainTensor), C.c_int32, C.c_int32, C.c_float, C.c_void_p, C.c_void_p,
                                          C.c_void_p]),

@@ -4,6 +4,10 @@
 #include "policy_loss_rows.cuh"
 
 namespace ob200 {
+
+static std::atomic<uint32_t> g_spin_limit{ptx::kSpinLimit};
+uint32_t policy_spin_limit() { return g_spin_limit.load(std::memory_order_relaxed); }
+
 namespace {
 
 using Rows = PolicyRows;
@@ -71,6 +75,8 @@ int launch_rows(int kind, const Rows& r, int dtype, cudaStream_t st) {
 using namespace ob200;
 
 extern "C" {
+
+void ob200_debug_policy_waits(int32_t give_up) { g_spin_limit.store(give_up ? 0u : ptx::kSpinLimit, std::memory_order_relaxed); }
 
 int ob200_launch_policy_loss_search(const ob200_policy_rows* rows, const void* target, int64_t target_pitch, int32_t target_kind,
                                     float entropy_coef, ob200_stream stream) {

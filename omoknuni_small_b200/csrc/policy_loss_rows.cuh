@@ -49,6 +49,7 @@ struct PolicyRows {
 int launch_policy_rows_f32(int kind, const PolicyRows& r, cudaStream_t st);
 int launch_policy_rows_bf16(int kind, const PolicyRows& r, cudaStream_t st);
 int launch_policy_rows_f16(int kind, const PolicyRows& r, cudaStream_t st);
+uint32_t policy_spin_limit();           // polls before a wait for a row gives up (policy_loss.cu)
 
 #ifdef __CUDACC__
 namespace {
@@ -382,6 +383,7 @@ policy_long_rows_kernel(const __grid_constant__ PolicyRows r) {
 struct RowShape {
     int seg;                            // vectors a CTA holds of a row
     int x_at, mask_at, slot_bytes;      // offsets in a slot, its size
+    uint32_t spins;
     int* error;
 };
 constexpr int kHeader = 32;             // weight, old log-probability, advantage, action; head, vectors, -, flags
@@ -849,6 +851,17 @@ __device__ __forceinline__ void copy_vectors(const PolicyRows& r, long long row,
     }
 }
 
+// What a team whose copy did not arrive leaves of its rows from `row` on: NaN, so that no update is made of them (rows of
+// weight 0 as ever).
+template <typename T>
+__device__ __noinline__ void lost_rows(const PolicyRows& r, long long row, long long step, int tid, int threads) {
+    for (; row < r.n; row += step) {
+        const float y = r.weight && r.weight[row] == 0.f ? 0.f : __int_as_float(0x7fc00000);
+        if (tid == 0) put_out(r, row, true, RowOut{y, make_float4(y, y, y, y)});
+        for (int j = tid; j < r.A; j += threads) ((T*)r.grad)[row * r.g_pitch + j] = from_f32<T>(y);
+    }
+}
+
 // ---- short rows --------------------------------------------------------------------
 // LANES lanes a row, 32 / LANES adjacent rows a warp; each warp has slots of its own and fills them itself.  While a warp waits
 // for its copies the SM's others work: with two slots a warp, and so half the warps, 65,536 x 362 took 90 us, with one 52.
@@ -898,7 +911,14 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
         const Part p{at_s + kHeader, at_s + sh.x_at, at_s + sh.mask_at, 0, pl.head, pl.vecs, 0, is ? pl.vecs : 0, pl.first_out, pl.last_out};
         float4 scalars;
         if (ALIKE) {
-            if (!ptx::mbar_wait_warp(full, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+            if (!ptx::mbar_wait_warp(full, parity, &abort_flag, sh.spins)) {
+                abort_flag = 1;
+                atomicExch(sh.error, 4);
+                int none = 0;
+                ptx::mbar_wait(full, parity, &none);             // what is in flight is waited for once more
+                lost_rows<T>(r, row, step, tid, LANES);
+                break;
+            }
             parity ^= 1;
             scalars = *(const float4*)at;
         } else {
@@ -958,10 +978,6 @@ policy_warp_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_const
             if (!apart) copy_out<T>(r, p, tid, LANES, grad);
             __syncwarp();
         }
-    }
-    if (ALIKE && abort_flag) {                   // a wait ran out: what is still in flight is waited for once more, within the same limit
-        int none = 0;
-        ptx::mbar_wait(full, parity ^ 1, &none);
     }
 }
 
@@ -1047,14 +1063,24 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
         if (first < r.n) fill(first, scalars_of(r, KIND, first));
         ahead = scalars_of(r, KIND, first + step);
     }
-    uint32_t parity = 0;
+    uint32_t parity = 0, filled = 0;             // of the row's barrier phase; of the last row filled
     int turn = 0;
     for (long long row = first; row < r.n; row += step) {
         float4 scalars;
         Place pl;
+        // The row's copy did not arrive, or an earlier one's: no slot is filled any more.  Its scalars, which all warps of a
+        // row have to agree on, come from where the slot has them from, and its sums are NaN.
+        bool lost = false;
         if (ALIKE) {
-            if (!ptx::mbar_wait_warp(full, parity, &abort_flag)) { abort_flag = 1; atomicExch(sh.error, 4); }
+            lost = __any_sync(~0u, *(volatile int*)&abort_flag);
+            if (!lost && !ptx::mbar_wait_warp(full, parity, &abort_flag, sh.spins)) {
+                lost = true;
+                abort_flag = 1;
+                atomicExch(sh.error, 4);
+            }
             parity ^= 1;
+        }
+        if (ALIKE && !lost) {
             scalars = *(const float4*)smem;
             const int4 h = *(const int4*)(smem + 16);
             pl = Place{h.x, h.y, (h.w & 1) != 0, (h.w & 2) != 0};
@@ -1076,9 +1102,9 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
         RowOut out;
         if (live) {                              // the same in the whole team
             Tops tops{Lowest<T>::kWord, Lowest<T>::kWord, Lowest<T>::kWord};
-            const bool some = __any_sync(~0u, pass_max<T, KIND, ALIKE, U, false>(r, row, p, threadIdx.x, threads, tops));
+            const bool some = __any_sync(~0u, pass_max<T, KIND, ALIKE, U, false>(r, row, p, threadIdx.x, threads, tops)) || lost;
             floored = std::is_same<T, __half>::value && __any_sync(~0u, has_minus_inf<T>(tops.low));
-            const float top = warp_max_nan(word_top<T>(tops.z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(tops.x)) : 0.f;
+            float top = warp_max_nan(word_top<T>(tops.z)), top_ref = KIND == kClippedRef ? warp_max_nan(word_top<T>(tops.x)) : 0.f;
             __syncwarp();
             // The action's logit, by the warp that has its vector and ahead of the meeting: behind it the others may find the
             // gradient in its place.
@@ -1091,7 +1117,8 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             q.c = KIND == kClippedRef ? base_of<T>(top_ref) : 0.f;
             if (floored) pass_sums<T, KIND, U, true>(p, threadIdx.x, threads, q);
             else pass_sums<T, KIND, U, false>(p, threadIdx.x, threads, q);
-            const float sum = four_sums(q.s, q.t, q.a, q.b);
+            float sum = four_sums(q.s, q.t, q.a, q.b);
+            if (lost) top = top_ref = sum = za = __int_as_float(0x7fc00000);
             float (*all)[8] = part[turn];
             turn ^= 1;
             float* const mine = all[cta * warps + warp];
@@ -1126,7 +1153,8 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             // the next copy comes behind what was read and written here
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncthreads();
-            if (warp == 0 && row + step < r.n) {
+            if (warp == 0 && row + step < r.n && !*(volatile int*)&abort_flag) {
+                filled ^= 1;
                 fill(row + step, ahead);
                 ahead = scalars_of(r, KIND, row + 2 * step);
             }
@@ -1136,9 +1164,9 @@ policy_cta_rows_kernel(const __grid_constant__ PolicyRows r, const __grid_consta
             __syncthreads();
         }
     }
-    if (ALIKE && abort_flag && threadIdx.x == 0) {       // a wait ran out: what is still in flight is waited for once more, within the same limit
+    if (ALIKE && abort_flag && threadIdx.x == 0) {       // what is still in flight is waited for once more
         int none = 0;
-        ptx::mbar_wait(full, parity ^ 1, &none);
+        ptx::mbar_wait(full, filled, &none);
     }
     __syncthreads();
     // and none may leave while another may still write
@@ -1230,6 +1258,7 @@ int launch_shape(const PolicyRows& r, cudaStream_t st) {
     const int vecs = (int)(((long long)r.A + (ALIKE ? V - 1 : 0) + V - 1) / V);
     RowShape sh{};
     sh.error = device_error_word();
+    sh.spins = policy_spin_limit();
     if (!sh.error) return set_error(OB200_ERR_CUDA, "policy loss: the device's error word is not available");
     auto lay = [&](int ctas) {
         sh.seg = (vecs + ctas - 1) / ctas;

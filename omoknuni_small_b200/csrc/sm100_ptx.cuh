@@ -41,8 +41,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // The same for a whole warp: every lane waits, and the answer is the warp's.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit = kSpinLimit) {
+    for (uint32_t i = 0; i < limit; ++i) {
         if (__all_sync(0xFFFFFFFFu, mbar_test(bar, parity))) return true;
         if ((i & 255) == 255 && __any_sync(0xFFFFFFFFu, *abort_flag)) return false;
     }

@@ -46,7 +46,8 @@ def batch_of(positions, board_size):
 
 class HeadLearner:
     """One optimiser over the heads of `net` (a finalised capi.Net for Gomoku) whose tensors are `weights`.  Steps run on
-    PyTorch's current stream and return without waiting; the handle may answer and search between them.
+    PyTorch's current stream and return without waiting; the handle may answer and search between them.  A kernel that gave
+    up on a wait makes its step's losses NaN and the step is left out; fit() and weights() report it.
 
     state_bits: AdamW states in 32 or 8 bits.  max_norm: the gradients' norm is clipped to it.  value_coef: factor of the
     squared error of the value.  The heads as they are at the start are the reference of the KL term of step_clipped."""
@@ -169,10 +170,20 @@ class HeadLearner:
             b = {k: torch.from_numpy(v).to(self.device) for k, v in b.items()}
             loss, value_loss, _, _ = self.step_search(b["history"], b["n_hist"], b["to_move"], b["target"], b["outcome"], b["legal_bits"], lr=lr)
             seen.append(torch.stack([loss.sum(), value_loss.sum()]))
-        return torch.stack(seen).cpu().numpy() if seen else np.zeros((0, 2), np.float32)
+        losses = torch.stack(seen).cpu().numpy() if seen else np.zeros((0, 2), np.float32)
+        self._reported()
+        return losses
 
     def weights(self):
         """Every tensor of the network under the reference's names, the heads as they are now (numpy float32)."""
         out = dict(self.all)
         out.update({k: p.detach().cpu().numpy().copy() for k, p in self.params.items()})
+        self._reported()
         return out
+
+    def _reported(self):
+        """Raises what a kernel that gave up on a wait has left on the device; steps it had a part in were left out."""
+        with self.torch.cuda.device(self.device):
+            code = capi.device_error_code()
+        if code:
+            raise capi.Error(capi.ERR_TIMEOUT, f"HeadLearner: a kernel gave up on a bounded wait (code {code})")
