@@ -44,6 +44,17 @@ def batch_of(positions, board_size):
     return dict(history=history, n_hist=n_hist, to_move=to_move, legal_bits=np.ascontiguousarray(bits), target=target, outcome=outcome)
 
 
+def check_positions(device, history, n_hist, to_move, outcome=None):
+    """Refuses what the encoder would read out of its bounds or as something else."""
+    import torch
+    n = history.shape[0] if history.dim() else 0
+    for t, what, shape, dtype in ((history, "history", (n, 16), torch.int16), (n_hist, "n_hist", (n,), torch.uint8), (to_move, "to_move", (n,), torch.uint8),
+                                  (outcome, "outcome", (n,), None)):
+        if t is not None and (tuple(t.shape) != shape or t.device != device or dtype not in (None, t.dtype) or (dtype and not t.is_contiguous())):
+            raise capi.Error(capi.ERR_INVALID, f"HeadLearner: {what} is {shape} of {dtype or 'numbers'} on {device}, got {tuple(t.shape)} of "
+                                               f"{t.dtype} on {t.device}")
+
+
 class HeadLearner:
     """One optimiser over the heads of `net` (a finalised capi.Net for Gomoku) whose tensors are `weights`.  Steps run on
     PyTorch's current stream and return without waiting; the handle may answer and search between them.  A kernel that gave
@@ -82,6 +93,7 @@ class HeadLearner:
 
     def features(self, history, n_hist, to_move):
         """Tower output [n, filters, S, S] float32 of positions given as device arrays (capi.encode_gomoku)."""
+        check_positions(self.device, history, n_hist, to_move)
         torch, S, n = self.torch, self.S, history.shape[0]
         channels = self.net.input_tensor_channels()
         if n > self.net.cfg.max_batch:
@@ -132,6 +144,7 @@ class HeadLearner:
         """One step towards the search's policies (`target`: visit counts int32, or float32) and the games' outcomes.
         Device arrays; row_weight [n] (default 1 / n), 0 for rows that fill up a batch.  Returns (loss of the policy rows
         [n], loss of the value rows [n], statistics of the policy rows [n, 4], (norm, factor)), all on the device."""
+        check_positions(self.device, history, n_hist, to_move, outcome)
         w = self._weight(history.shape[0], row_weight)
         with self.torch.cuda.device(self.device):
             logits, value = self.heads(self.features(history, n_hist, to_move))
@@ -144,6 +157,7 @@ class HeadLearner:
                      kl_coef=0.0, lr=1e-3):
         """One step of the clipped-ratio objective on moves that were played: `old_logp` is the log-probability with which
         each was drawn; kl_coef holds the policy to that of the heads the learner started with.  Returns as step_search."""
+        check_positions(self.device, history, n_hist, to_move, outcome)
         w = self._weight(history.shape[0], row_weight)
         with self.torch.cuda.device(self.device):
             x = self.features(history, n_hist, to_move)
