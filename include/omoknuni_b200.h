@@ -806,8 +806,8 @@ typedef struct ob200_adamw_config {
  * value above 0 never becoming 0.  The step itself uses m and v before they are
  * rounded.  Zeroed codes and scales are the state before the first step.
  * A moment that is not finite makes the states of its 256 elements NaN.
- * No two tensors of a call may share memory (OB200_ERR_INVALID where params or
- * states of one kind do). */
+ * Nothing that a call writes (params, states, scales, of one tensor or of two) may
+ * share memory (OB200_ERR_INVALID where it does); nor may a gradient with it. */
 int ob200_launch_adamw(const ob200_train_tensor* tensors, int32_t n_tensors, const ob200_adamw_config* cfg,
                        ob200_stream stream);
 

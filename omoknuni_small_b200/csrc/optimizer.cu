@@ -8,6 +8,7 @@
 #include "packed_f32.cuh"
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <memory>
 #include <new>
 #include <cuda_bf16.h>
@@ -461,24 +462,45 @@ int adamw_param(const ob200_train_tensor* tensors, int n, const ob200_adamw_conf
     return adamw_typed<P, float>(tensors, n, c->state_bits, k, st);
 }
 
-// Whether two entries share memory of one kind (`base`, es bytes an element): two CTAs would update it at once.
-int check_apart(const char* who, const ob200_train_tensor* t, int n, int es, void* ob200_train_tensor::*base, const char* what) {
-    auto begin = [&](int i) { return (uintptr_t)(t[i].*base); };
-    auto end = [&](int i) { return begin(i) + (uintptr_t)t[i].numel * es; };
-    uintptr_t last = 0;
+// Memory of one kind that a call writes: `bytes` for every 2^shift elements of a tensor (scales: a float for 256).
+struct Written { const char* what; size_t at; int bytes, shift; };       // at: the pointer's place in an ob200_train_tensor
+// Whether two tensors of a call share memory that it writes: two CTAs would update it at once.
+int check_apart(const char* who, const ob200_train_tensor* t, int n, const Written* kinds, int n_kinds) {
+    auto begin = [&](const Written& k, int i) {
+        uintptr_t at;
+        std::memcpy(&at, (const char*)(t + i) + k.at, sizeof(at));
+        return at;
+    };
+    auto end = [&](const Written& k, int i) { return begin(k, i) + (uintptr_t)((t[i].numel + (1 << k.shift) - 1) >> k.shift) * k.bytes; };
+    // in the order of memory, as the views of flat buffers are, each kind in a buffer of its own
+    uintptr_t lo[5], hi[5];
     bool apart = true;
-    for (int i = 0; i < n && apart; ++i)
-        if (t[i].numel) { apart = begin(i) >= last; last = end(i); }
-    if (apart) return OB200_OK;           // in the order of memory, as the views of a flat buffer are
-    std::unique_ptr<int[]> order(new (std::nothrow) int[n]);
-    if (!order) return set_error(OB200_ERR_STATE, "%s: out of host memory", who);
-    int k = 0;
-    for (int i = 0; i < n; ++i)
-        if (t[i].numel) order[k++] = i;
-    std::sort(order.get(), order.get() + k, [&](int a, int b) { return begin(a) < begin(b); });
-    for (int i = 1; i < k; ++i)
-        if (begin(order[i]) < end(order[i - 1]))
-            return set_error(OB200_ERR_INVALID, "%s: tensors %d and %d share memory (%s)", who, order[i - 1], order[i], what);
+    for (int k = 0; k < n_kinds && apart; ++k) {
+        const Written kind = kinds[k];
+        uintptr_t first = 0, last = 0;
+        for (int i = 0; i < n && apart; ++i) {
+            if (!t[i].numel) continue;
+            const uintptr_t at = begin(kind, i);
+            if (!last) first = at;
+            else apart = at >= last;
+            last = end(kind, i);
+        }
+        lo[k] = first; hi[k] = last;
+        for (int q = 0; q < k && apart; ++q) apart = hi[k] <= lo[q] || hi[q] <= lo[k];
+    }
+    if (apart) return OB200_OK;
+    struct Span { uintptr_t begin, end; int kind, i; };
+    std::unique_ptr<Span[]> all(new (std::nothrow) Span[(size_t)n * n_kinds]);
+    if (!all) return set_error(OB200_ERR_STATE, "%s: out of host memory", who);
+    size_t count = 0;
+    for (int k = 0; k < n_kinds; ++k)
+        for (int i = 0; i < n; ++i)
+            if (t[i].numel) all[count++] = Span{begin(kinds[k], i), end(kinds[k], i), k, i};
+    std::sort(all.get(), all.get() + count, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    for (size_t s = 1; s < count; ++s)
+        if (all[s].begin < all[s - 1].end)
+            return set_error(OB200_ERR_INVALID, "%s: %s of tensor %d and %s of tensor %d share memory", who, kinds[all[s - 1].kind].what,
+                             all[s - 1].i, kinds[all[s].kind].what, all[s].i);
     return OB200_OK;
 }
 
@@ -533,9 +555,12 @@ int ob200_launch_adamw(const ob200_train_tensor* tensors, int32_t n_tensors, con
             (se == 1 && ((uintptr_t)t.exp_avg_scale | (uintptr_t)t.exp_avg_sq_scale) % 4))
             return set_error(OB200_ERR_INVALID, "%s: tensor %d is not aligned", who, i);
     }
-    if (int rc = check_apart(who, tensors, n_tensors, pe, &ob200_train_tensor::param, "param")) return rc;
-    if (int rc = check_apart(who, tensors, n_tensors, se, &ob200_train_tensor::exp_avg, "exp_avg")) return rc;
-    if (int rc = check_apart(who, tensors, n_tensors, se, &ob200_train_tensor::exp_avg_sq, "exp_avg_sq")) return rc;
+    using Tensor = ob200_train_tensor;
+    const Written kinds[5] = {{"param", offsetof(Tensor, param), pe, 0}, {"exp_avg", offsetof(Tensor, exp_avg), se, 0},
+                              {"exp_avg_sq", offsetof(Tensor, exp_avg_sq), se, 0}, {"exp_avg_scale", offsetof(Tensor, exp_avg_scale), 4, 8},
+                              {"exp_avg_sq_scale", offsetof(Tensor, exp_avg_sq_scale), 4, 8}};
+    static_assert(kBlock == 1 << 8, "a scale's elements");
+    if (int rc = check_apart(who, tensors, n_tensors, kinds, se == 1 ? 5 : 3)) return rc;
     if (int rc = require_device()) return rc;
     Step k{};
     const double b1 = c->beta1, b2 = c->beta2;
