@@ -713,7 +713,8 @@ typedef struct ob200_policy_rows {
                                    itself (same pitch)                            */
     float* loss;                /* [n], or NULL                                   */
     float* stats;               /* [n][4], 16-byte aligned, or NULL               */
-    int64_t logits_pitch;       /* elements between rows, n_actions to 2^31       */
+    int64_t logits_pitch;       /* elements between rows, n_actions to 2^31; a matrix
+                                   has at most 2^46 elements                      */
     int64_t grad_pitch;
     int32_t n;                  /* rows; 0 is a call without work                 */
     int32_t n_actions;          /* 1 to 2^30                                      */

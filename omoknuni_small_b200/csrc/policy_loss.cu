@@ -24,8 +24,8 @@ bool rows_meet(const void* a, long long pa, int ea, const void* b, long long pb,
     return off < A * ea || off + A * eb > step;
 }
 
-// Pitches are at most 2^31, so that no offset of n rows leaves 64 bits.
-bool pitch_fits(long long pitch, int A) { return pitch >= A && pitch <= 1LL << 31; }
+// A matrix ends within 2^46 elements of its start: beyond any memory, and no offset in bytes leaves 64 bits.
+bool pitch_fits(long long pitch, int A, int n) { return pitch >= A && pitch <= 1LL << 31 && (n - 1LL) * pitch + A <= 1LL << 46; }
 
 // What both losses ask of their rows; fills the shared part of r.
 int take_rows(const char* who, const ob200_policy_rows* p, Rows* r) {
@@ -37,12 +37,13 @@ int take_rows(const char* who, const ob200_policy_rows* p, Rows* r) {
     if (p->n == 0) return OB200_OK;
     const int es = elem_bytes(p->dtype);
     if (!p->logits || !p->grad) return set_error(OB200_ERR_INVALID, "%s: null logits or grad", who);
-    if (!pitch_fits(p->logits_pitch, p->n_actions) || !pitch_fits(p->grad_pitch, p->n_actions))
-        return set_error(OB200_ERR_INVALID, "%s: a pitch is below n_actions, or above 2^31", who);
+    if (!pitch_fits(p->logits_pitch, p->n_actions, p->n) || !pitch_fits(p->grad_pitch, p->n_actions, p->n))
+        return set_error(OB200_ERR_INVALID, "%s: a pitch is below n_actions or above 2^31, or a matrix beyond 2^46 elements", who);
     if (((uintptr_t)p->logits | (uintptr_t)p->grad) % es || ((uintptr_t)p->legal_bits | (uintptr_t)p->row_weight | (uintptr_t)p->loss) % 4 || (uintptr_t)p->stats % 16)
         return set_error(OB200_ERR_INVALID, "%s: a pointer is not aligned", who);
     if (p->legal_bits && p->mask_words < (p->n_actions + 31) / 32)
         return set_error(OB200_ERR_INVALID, "%s: mask_words %d too small for %d actions", who, p->mask_words, p->n_actions);
+    if (p->legal_bits && (long long)p->n * p->mask_words > 1LL << 46) return set_error(OB200_ERR_INVALID, "%s: legal_bits beyond 2^46 words", who);
     if (!(p->grad == p->logits && p->grad_pitch == p->logits_pitch) &&
         rows_meet(p->grad, p->grad_pitch, es, p->logits, p->logits_pitch, es, p->n, p->n_actions))
         return set_error(OB200_ERR_INVALID, "%s: grad overlaps logits (it may be logits itself, with the same pitch)", who);
@@ -86,8 +87,8 @@ int ob200_launch_policy_loss_search(const ob200_policy_rows* rows, const void* t
     if (target_kind != OB200_TARGET_VISITS && target_kind != OB200_TARGET_PROBS)
         return set_error(OB200_ERR_INVALID, "%s: bad target_kind %d", who, target_kind);
     if (rows->n > 0) {
-        if (!target || (uintptr_t)target % 4 || !pitch_fits(target_pitch, r.A))
-            return set_error(OB200_ERR_INVALID, "%s: target is null, not aligned, or its pitch is below n_actions", who);
+        if (!target || (uintptr_t)target % 4 || !pitch_fits(target_pitch, r.A, r.n))
+            return set_error(OB200_ERR_INVALID, "%s: target is null, not aligned, its pitch is below n_actions, or it goes too far", who);
         if (rows_meet(r.grad, r.g_pitch, elem_bytes(rows->dtype), target, target_pitch, 4, r.n, r.A))
             return set_error(OB200_ERR_INVALID, "%s: grad overlaps target", who);
     }
@@ -112,8 +113,8 @@ int ob200_launch_policy_loss_clipped(const ob200_policy_rows* rows, const int32_
             return set_error(OB200_ERR_INVALID, "%s: action, old_logp or advantage is null or not aligned", who);
         if (ref_logits) {
             const int es = elem_bytes(rows->dtype);
-            if ((uintptr_t)ref_logits % es || !pitch_fits(ref_pitch, r.A))
-                return set_error(OB200_ERR_INVALID, "%s: ref_logits is not aligned or its pitch is below n_actions", who);
+            if ((uintptr_t)ref_logits % es || !pitch_fits(ref_pitch, r.A, r.n))
+                return set_error(OB200_ERR_INVALID, "%s: ref_logits is not aligned, its pitch is below n_actions, or it goes too far", who);
             if (rows_meet(r.grad, r.g_pitch, es, ref_logits, ref_pitch, es, r.n, r.A))
                 return set_error(OB200_ERR_INVALID, "%s: grad overlaps ref_logits", who);
         }
