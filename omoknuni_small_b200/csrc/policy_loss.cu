@@ -54,6 +54,33 @@ int take_rows(const char* who, const ob200_policy_rows* p, Rows* r) {
     return OB200_OK;
 }
 
+// Whether `bytes` at v share a byte with rows [n][A] of es-byte elements at m.
+bool vector_meets(const void* v, long long bytes, const void* m, long long pitch, int es, long long n, long long A) {
+    const intptr_t v0 = (intptr_t)v, m0 = (intptr_t)m;
+    if (!v || !m || v0 + bytes <= m0 || m0 + ((n - 1) * pitch + A) * es <= v0) return false;
+    const intptr_t step = pitch * es, off = (((v0 - m0) % step) + step) % step;
+    return off < A * es || off + bytes > step;
+}
+
+// What a call writes shares no memory with what it reads, or with what else it writes (grad and the matrices it reads: take_rows
+// and the entry points).  x: target or reference logits.
+int check_vectors(const char* who, const Rows& r, int es, int x_bytes) {
+    struct Vector { const char* what; const void* at; long long bytes; };
+    const long long n = r.n;
+    const Vector v[7] = {{"loss", r.loss, 4 * n}, {"stats", r.stats, 16 * n}, {"row_weight", r.weight, 4 * n}, {"action", r.action, 4 * n},
+                         {"old_logp", r.old_logp, 4 * n}, {"advantage", r.advantage, 4 * n}, {"legal_bits", r.bits, 4 * n * r.mask_words}};
+    for (int i = 0; i < 7; ++i) {
+        if (vector_meets(v[i].at, v[i].bytes, r.grad, r.g_pitch, es, n, r.A)) return set_error(OB200_ERR_INVALID, "%s: grad overlaps %s", who, v[i].what);
+        if (i >= 2) continue;
+        if (vector_meets(v[i].at, v[i].bytes, r.z, r.z_pitch, es, n, r.A) || vector_meets(v[i].at, v[i].bytes, r.x, r.x_pitch, x_bytes, n, r.A))
+            return set_error(OB200_ERR_INVALID, "%s: %s overlaps a matrix", who, v[i].what);
+        for (int j = i + 1; j < 7; ++j)
+            if (v[i].at && v[j].at && (intptr_t)v[i].at < (intptr_t)v[j].at + v[j].bytes && (intptr_t)v[j].at < (intptr_t)v[i].at + v[i].bytes)
+                return set_error(OB200_ERR_INVALID, "%s: %s overlaps %s", who, v[i].what, v[j].what);
+    }
+    return OB200_OK;
+}
+
 // Whether the rows of all matrices start at the same element of a vector; then that of row 0.
 void find_phase(Rows* r, int dtype, int x_bytes) {
     const int es = elem_bytes(dtype), V = 16 / es;
@@ -91,10 +118,12 @@ int ob200_launch_policy_loss_search(const ob200_policy_rows* rows, const void* t
             return set_error(OB200_ERR_INVALID, "%s: target is null, not aligned, its pitch is below n_actions, or it goes too far", who);
         if (rows_meet(r.grad, r.g_pitch, elem_bytes(rows->dtype), target, target_pitch, 4, r.n, r.A))
             return set_error(OB200_ERR_INVALID, "%s: grad overlaps target", who);
+        r.x = target; r.x_pitch = target_pitch;
+        if (int rc = check_vectors(who, r, elem_bytes(rows->dtype), 4)) return rc;
     }
     if (int rc = require_device()) return rc;
     if (rows->n == 0) return OB200_OK;
-    r.x = target; r.x_pitch = target_pitch; r.entropy = entropy_coef;
+    r.entropy = entropy_coef;
     r.visits = target_kind == OB200_TARGET_VISITS;
     find_phase(&r, rows->dtype, 4);
     return launch_rows(kSearch, r, rows->dtype, as_stream(stream));
@@ -118,11 +147,12 @@ int ob200_launch_policy_loss_clipped(const ob200_policy_rows* rows, const int32_
             if (rows_meet(r.grad, r.g_pitch, es, ref_logits, ref_pitch, es, r.n, r.A))
                 return set_error(OB200_ERR_INVALID, "%s: grad overlaps ref_logits", who);
         }
+        r.x = ref_logits; r.x_pitch = ref_pitch;
+        r.action = action; r.old_logp = old_logp; r.advantage = advantage;
+        if (int rc = check_vectors(who, r, elem_bytes(rows->dtype), elem_bytes(rows->dtype))) return rc;
     }
     if (int rc = require_device()) return rc;
     if (rows->n == 0) return OB200_OK;
-    r.x = ref_logits; r.x_pitch = ref_pitch;
-    r.action = action; r.old_logp = old_logp; r.advantage = advantage;
     r.lo = 1.f - clip_low; r.hi = 1.f + clip_high; r.kl = kl_coef; r.entropy = entropy_coef;
     find_phase(&r, rows->dtype, elem_bytes(rows->dtype));
     return launch_rows(ref_logits ? kClippedRef : kClipped, r, rows->dtype, as_stream(stream));
