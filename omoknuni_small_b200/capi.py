@@ -648,18 +648,20 @@ def _train_dtype(dtype, what):
 
 
 def _launch_on(device, fn, *args):
-    """fn(*args, stream) with the tensors' device as the current one, on its current stream."""
+    """fn(*args, stream) with the tensors' device as the current one, on its current stream, which is returned."""
     import torch
     if device.type != "cuda":
         _refuse("the tensors are not on a CUDA device (there is no CPU path)")
     raw, index = torch._C._cuda_getCurrentRawStream, device.index      # what torch.cuda.current_stream() wraps, a tenth of its time
+    stream = raw(index)
     if index == torch._C._cuda_getDevice():
-        rc = fn(*args, raw(index))
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, raw(index))
+            rc = fn(*args, stream)
     if rc != 0:
         check(rc)
+    return stream
 
 
 def _pitch(t, what, n, A, device, dtype):
@@ -753,10 +755,29 @@ def _cleared(make, device, what):
     return made
 
 
-class GradNorm:
+class _Plan:
+    """What keeps memory of its own for calls on any stream: `_own`, allocated on the stream `_home`."""
+
+    def _keep(self, tensors):
+        import torch
+        self._own, self._home, self._seen = tensors, torch._C._cuda_getCurrentRawStream(self.device.index), set()
+
+    def _ran_on(self, stream):
+        """Tells the allocator of another stream, so that dropping the plan does not hand its memory out while that still runs."""
+        if stream == self._home or stream in self._seen:
+            return
+        import torch
+        self._seen.add(stream)
+        current = torch.cuda.current_stream(self.device)
+        for t in self._own:
+            t.record_stream(current)
+
+
+class GradNorm(_Plan):
     """2-norm over a fixed list of gradients and the factor that clips it (ob200_launch_grad_norm).  run(max_norm) fills
     and returns `out` (float32 [2] on the device: norm, factor); `clip` is the factor as AdamW.step takes it.  The plan
-    keeps the gradients and its workspace: one plan per stream that runs at the same time."""
+    keeps the gradients and its workspace: one plan per stream that runs at the same time.  It may be dropped while a call
+    runs; a graph that captured one needs the plan as long as it is replayed."""
 
     def __init__(self, grads, out=None):
         import torch
@@ -770,17 +791,18 @@ class GradNorm:
         _require(self.out.dtype == torch.float32 and self.out.device == self.device and tuple(self.out.shape) == (2,)
                  and self.out.is_contiguous(), "GradNorm: out is float32 [2] on the gradients' device")
         self.clip = self.out[1:]
+        self._keep([self.workspace] + ([self.out] if out is None else []))
         self.table = (TrainTensor * len(self.grads))()
         for e, g in zip(self.table, self.grads):
             e.grad, e.numel = g.data_ptr(), g.numel()
 
     def run(self, max_norm=float("inf")):
-        _launch_on(self.device, lib().ob200_launch_grad_norm, self.table, len(self.table), self.dtype, max_norm, self.workspace.data_ptr(),
-                   self.out.data_ptr())
+        self._ran_on(_launch_on(self.device, lib().ob200_launch_grad_norm, self.table, len(self.table), self.dtype, max_norm,
+                                self.workspace.data_ptr(), self.out.data_ptr()))
         return self.out
 
 
-class AdamW:
+class AdamW(_Plan):
     """AdamW over a fixed list of weights and gradients, one launch a step (ob200_launch_adamw).
 
     params, grads: contiguous tensors of one float type each on one device; the gradients' buffers are kept, so whatever
@@ -812,7 +834,8 @@ class AdamW:
 
         def size(p, per):
             return (p.numel() + per - 1) // per
-        if state is None:
+        given = state is not None
+        if not given:
             state = _cleared(lambda: {k: [torch.zeros(size(p, per), dtype=torch.uint8 if dt == torch.float8_e4m3fn else dt, device=self.device).view(dt)
                                           for p in self.params] for k, (dt, per) in keys.items()}, self.device, "AdamW")
         self.state = {k: list(state[k]) if k in state else None for k in keys}
@@ -827,6 +850,7 @@ class AdamW:
             for k in keys:
                 setattr(e, k, self.state[k][i].data_ptr())
         self.cfg = AdamWConfig(beta1=betas[0], beta2=betas[1], eps=eps, param_dtype=p_dtype, grad_dtype=g_dtype, state_bits=state_bits)
+        self._keep([] if given else [t for ts in self.state.values() for t in ts])
         self.steps = 0
 
     def _scalar(self, t, what, dtype):
@@ -849,6 +873,6 @@ class AdamW:
             c.step, c.step_device = 0, self._scalar(step, "step", torch.int32)
         else:
             c.step, c.step_device = self.steps + 1 if step is None else step, None
-        _launch_on(self.device, lib().ob200_launch_adamw, self.table, len(self.table), c)
+        self._ran_on(_launch_on(self.device, lib().ob200_launch_adamw, self.table, len(self.table), c))
         if c.step:
             self.steps = c.step
