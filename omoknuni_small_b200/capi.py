@@ -6,6 +6,7 @@ fallback implementation.
 """
 import ctypes as C
 import os
+import threading
 
 import numpy as np
 
@@ -809,7 +810,8 @@ class AdamW(_Plan):
     fills them has to write in place.  state_bits: 32, or 8 (e4m3 codes with a float32 scale per 256 elements).
     weight_decay: a number, or one per tensor.  state: {"exp_avg": [...], "exp_avg_sq": [...]} and for 8 bits
     {"exp_avg_scale": [...], "exp_avg_sq_scale": [...]} to go on from, zeros otherwise; it is `self.state`, updated in
-    place.  `self.steps` counts the steps made."""
+    place.  `self.steps` is the count of the last step that was counted on the host.  Steps from several threads are launched one
+    after the other."""
 
     BLOCK = 256
 
@@ -849,6 +851,7 @@ class AdamW(_Plan):
             e.param, e.grad, e.numel, e.weight_decay = self.params[i].data_ptr(), self.grads[i].data_ptr(), self.params[i].numel(), decay[i]
             for k in keys:
                 setattr(e, k, self.state[k][i].data_ptr())
+        self._lock = threading.Lock()        # cfg and steps are a step's own while it is launched
         self.cfg = AdamWConfig(beta1=betas[0], beta2=betas[1], eps=eps, param_dtype=p_dtype, grad_dtype=g_dtype, state_bits=state_bits)
         self._keep([] if given else [t for ts in self.state.values() for t in ts])
         self.steps = 0
@@ -863,16 +866,17 @@ class AdamW(_Plan):
         int32 scalar on the device - for captured graphs, nothing is changed while it is below 1; grad_scale: a float32 scalar on the device that multiplies every
         gradient (GradNorm.clip); when it is not finite weights and states stay as they are, while the count goes on."""
         import torch
-        c = self.cfg
-        c.grad_scale = None if grad_scale is None else self._scalar(grad_scale, "grad_scale", torch.float32)
-        if isinstance(lr, torch.Tensor):
-            c.lr, c.lr_device = 0.0, self._scalar(lr, "lr", torch.float32)
-        else:
-            c.lr, c.lr_device = lr, None
-        if isinstance(step, torch.Tensor):
-            c.step, c.step_device = 0, self._scalar(step, "step", torch.int32)
-        else:
-            c.step, c.step_device = self.steps + 1 if step is None else step, None
-        self._ran_on(_launch_on(self.device, lib().ob200_launch_adamw, self.table, len(self.table), c))
-        if c.step:
-            self.steps = c.step
+        with self._lock:
+            c = self.cfg
+            c.grad_scale = None if grad_scale is None else self._scalar(grad_scale, "grad_scale", torch.float32)
+            if isinstance(lr, torch.Tensor):
+                c.lr, c.lr_device = 0.0, self._scalar(lr, "lr", torch.float32)
+            else:
+                c.lr, c.lr_device = lr, None
+            if isinstance(step, torch.Tensor):
+                c.step, c.step_device = 0, self._scalar(step, "step", torch.int32)
+            else:
+                c.step, c.step_device = self.steps + 1 if step is None else step, None
+            self._ran_on(_launch_on(self.device, lib().ob200_launch_adamw, self.table, len(self.table), c))
+            if c.step:
+                self.steps = c.step
