@@ -335,7 +335,8 @@ adamw_kernel(const __grid_constant__ Table<N> t, const __grid_constant__ Step k)
         // both reciprocals in one, a lane each
         const float top = lane & 1 ? r_top : m_top, ratio = __fmul_rn(__frcp_rn(top), kE4m3Max);
         const float mi = __shfl_sync(~0u, ratio, 0), ri = __shfl_sync(~0u, ratio, 1);
-        if (lane < 2) (lane ? e.vs : e.ms)[first + b] = __fmul_rn(top, 1.f / kE4m3Max);
+        // an infinite maximum's scale is NaN, else a root above 0 would be infinite and its weight stand still
+        if (lane < 2) (lane ? e.vs : e.ms)[first + b] = __fmul_rn(top + (top - top), 1.f / kE4m3Max);
         const f32x2 mi2 = pair(mi, mi), ri2 = pair(ri, ri);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
