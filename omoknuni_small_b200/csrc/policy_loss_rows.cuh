@@ -1181,9 +1181,10 @@ constexpr int kMostShared = 208 * 1024;          // of a CTA; 227 KB less the ke
 // memory.
 struct KernelFacts { std::atomic<int> of[64]; };
 template <typename Kernel>
-int kernel_facts(Kernel kernel, KernelFacts* known, int* facts) {
+int kernel_facts(Kernel kernel, KernelFacts* known, int* facts, int* device = nullptr) {
     int dev = 0, sms = 0;
     OB200_CUDA_OK(cudaGetDevice(&dev));
+    if (device) *device = dev;
     if (dev < 64 && (*facts = known->of[dev].load(std::memory_order_acquire)) != 0) return OB200_OK;
     cudaFuncAttributes a;
     OB200_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
@@ -1219,8 +1220,8 @@ template <typename T, int KIND, bool ALIKE>
 int launch_cta_rows(const PolicyRows& r, const RowShape& sh, int warps, int ctas, cudaStream_t st) {
     static KernelFacts known;
     auto kernel = policy_cta_rows_kernel<T, KIND, ALIKE>;
-    int facts;
-    if (int rc = kernel_facts(kernel, &known, &facts)) return rc;
+    int facts, dev;
+    if (int rc = kernel_facts(kernel, &known, &facts, &dev)) return rc;
     const int threads = 32 * warps, smem = sh.slot_bytes;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1233,10 +1234,10 @@ int launch_cta_rows(const PolicyRows& r, const RowShape& sh, int warps, int ctas
     if (ctas > 1) {
         // Fewer clusters fit than their CTAs would: not every group of SMs divides into them.  Each cluster has its share of
         // the rows, so one that had to wait for another's end would double the time.  The answer is kept for the next call
-        // with the same shape.
+        // with the same shape on the same device.
         static std::atomic<uint64_t> last[4];
         std::atomic<uint64_t>& slot = last[ctas == 2 ? 0 : ctas == 4 ? 1 : 2];
-        const uint64_t key = (uint64_t)smem << 32 | (uint64_t)threads << 16;
+        const uint64_t key = (uint64_t)dev << 52 | (uint64_t)smem << 32 | (uint64_t)threads << 16;
         uint64_t got = slot.load(std::memory_order_relaxed);
         if ((got & ~0xFFFFULL) != key) {
             int n = 0;
