@@ -782,7 +782,7 @@ int ob200_launch_grad_norm(const ob200_train_tensor* tensors, int32_t n_tensors,
                            void* workspace, float* out, ob200_stream stream);
 
 typedef struct ob200_adamw_config {
-    double lr, beta1, beta2, eps;
+    double lr, beta1, beta2, eps;   /* betas in [0, 1); eps 0 or at least 2^-126      */
     int32_t step;               /* 1 for the first step                           */
     int32_t param_dtype;        /* OB200_DTYPE_*                                  */
     int32_t grad_dtype;

@@ -542,6 +542,8 @@ int ob200_launch_adamw(const ob200_train_tensor* tensors, int32_t n_tensors, con
     if (c->state_bits != 8 && c->state_bits != 32) return set_error(OB200_ERR_INVALID, "%s: state_bits is 8 or 32, got %d", who, c->state_bits);
     if (!(c->beta1 >= 0.0 && c->beta1 < 1.0 && c->beta2 >= 0.0 && c->beta2 < 1.0 && c->eps >= 0.0))
         return set_error(OB200_ERR_INVALID, "%s: beta1 and beta2 are in [0, 1), eps is not negative", who);
+    if ((float)c->eps > 0.f && (float)c->eps < 0x1p-126f)        // the reciprocal of a subnormal sum is infinite, times a moment of 0 NaN
+        return set_error(OB200_ERR_INVALID, "%s: eps is 0 or at least 2^-126 in fp32", who);
     if (!c->step_device && c->step < 1) return set_error(OB200_ERR_INVALID, "%s: step counts from 1, got %d", who, c->step);
     if (((uintptr_t)c->grad_scale | (uintptr_t)c->lr_device | (uintptr_t)c->step_device) % 4)
         return set_error(OB200_ERR_INVALID, "%s: grad_scale, lr_device or step_device is not aligned", who);

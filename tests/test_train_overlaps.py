@@ -62,3 +62,9 @@ def test_adamw_memory_that_is_written_twice(api, bits, order):
         t = three()
         t[0].exp_avg_scale = t[1].param
         assert allowed(adamw(api, t, 3, bits))
+
+
+def test_eps_that_is_subnormal(api):
+    """Its reciprocal would be infinite where a second moment is 0, and the weight beside a zero gradient NaN."""
+    for eps in (1e-38, 1e-40, 2.0 ** -149):
+        assert api.lib().ob200_launch_adamw(tensors(api), 2, C.byref(config(api, eps=eps)), None) == api.ERR_INVALID
