@@ -238,3 +238,30 @@ def test_very_large_logits(api, dt, A):
     assert stats[0, 1] == 0 and abs(stats[1, 1] - math.log(A - 1)) <= 4 * D * (1 + math.log(A))
     assert abs(grad[0, 3] - (A - 1) / A) <= 4 * D + half and (np.abs(grad[0, 4:] + 1 / A) <= (4 * D + half) / A).all()
     assert abs(grad[1, 3] + 1 / A) <= (4 * D + half) / A
+
+
+@pytest.mark.parametrize("where", ["logits", "reference"])
+@pytest.mark.parametrize("A", LENGTHS)
+@pytest.mark.parametrize("dt", TYPES)
+def test_plus_infinity_makes_its_row_nan(api, dt, A, where):
+    """A legal +inf, of the logits or the reference, makes loss, gradient and the statistics that depend on it NaN; at an
+    action that is not legal it does not matter."""
+    import torch
+    n, T = 9, dtype_of(dt)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(A)
+    z, zr = torch.randn((2, n, A), generator=g, device="cuda").to(T)
+    x = z if where == "logits" else zr
+    x[::3, A // 2] = INF
+    x[1::3, A - 1] = INF
+    legal = np.ones((n, A), bool)
+    legal[1::3, A - 1] = False
+    act, one = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.ones(n, device="cuda")
+    for kappa in (0.0, 0.5):
+        loss, grad, stats = api.policy_loss_clipped(z, act, -one, one, pack(legal), zr, kl_coef=kappa, entropy_coef=0.1)
+        bad = torch.arange(n, device="cuda") % 3 == 0
+        assert torch.isnan(loss[bad]).all() and torch.isnan(grad[bad]).all() and torch.isnan(stats[bad, 2]).all()
+        assert torch.isfinite(loss[~bad]).all() and torch.isfinite(grad[~bad]).all() and torch.isfinite(stats[~bad]).all()
+    if where == "logits":
+        loss, grad, stats = api.policy_loss_search(z, torch.rand((n, A), generator=g, device="cuda"), pack(legal))
+        assert torch.isnan(loss[bad]).all() and torch.isnan(grad[bad]).all() and torch.isfinite(grad[~bad]).all() and torch.isfinite(loss[~bad]).all()
