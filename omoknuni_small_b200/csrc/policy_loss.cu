@@ -54,28 +54,27 @@ int take_rows(const char* who, const ob200_policy_rows* p, Rows* r) {
     return OB200_OK;
 }
 
-// Whether `bytes` at v share a byte with rows [n][A] of es-byte elements at m.
-bool vector_meets(const void* v, long long bytes, const void* m, long long pitch, int es, long long n, long long A) {
-    const intptr_t v0 = (intptr_t)v, m0 = (intptr_t)m;
-    if (!v || !m || v0 + bytes <= m0 || m0 + ((n - 1) * pitch + A) * es <= v0) return false;
-    const intptr_t step = pitch * es, off = (((v0 - m0) % step) + step) % step;
-    return off < A * es || off + bytes > step;
-}
-
 // What a call writes shares no memory with what it reads, or with what else it writes (grad and the matrices it reads: take_rows
 // and the entry points).  x: target or reference logits.
 int check_vectors(const char* who, const Rows& r, int es, int x_bytes) {
-    struct Vector { const char* what; const void* at; long long bytes; };
-    const long long n = r.n;
-    const Vector v[7] = {{"loss", r.loss, 4 * n}, {"stats", r.stats, 16 * n}, {"row_weight", r.weight, 4 * n}, {"action", r.action, 4 * n},
-                         {"old_logp", r.old_logp, 4 * n}, {"advantage", r.advantage, 4 * n}, {"legal_bits", r.bits, 4 * n * r.mask_words}};
+    struct Vector { const char* what; const void* at; long long unit; };
+    const Vector v[7] = {{"loss", r.loss, 4}, {"stats", r.stats, 16}, {"row_weight", r.weight, 4}, {"action", r.action, 4},
+                         {"old_logp", r.old_logp, 4}, {"advantage", r.advantage, 4}, {"legal_bits", r.bits, 4LL * r.mask_words}};
+    const struct Matrix { intptr_t at, step, row; } m[3] = {{(intptr_t)r.grad, (intptr_t)r.g_pitch * es, (intptr_t)r.A * es},
+                                                            {(intptr_t)r.z, (intptr_t)r.z_pitch * es, (intptr_t)r.A * es},
+                                                            {(intptr_t)r.x, (intptr_t)r.x_pitch * x_bytes, (intptr_t)r.A * x_bytes}};
+    intptr_t end[3];
+    for (int k = 0; k < 3; ++k) end[k] = m[k].at + (m[k].at ? (r.n - 1) * m[k].step + m[k].row : 0);
     for (int i = 0; i < 7; ++i) {
-        if (vector_meets(v[i].at, v[i].bytes, r.grad, r.g_pitch, es, n, r.A)) return set_error(OB200_ERR_INVALID, "%s: grad overlaps %s", who, v[i].what);
-        if (i >= 2) continue;
-        if (vector_meets(v[i].at, v[i].bytes, r.z, r.z_pitch, es, n, r.A) || vector_meets(v[i].at, v[i].bytes, r.x, r.x_pitch, x_bytes, n, r.A))
-            return set_error(OB200_ERR_INVALID, "%s: %s overlaps a matrix", who, v[i].what);
-        for (int j = i + 1; j < 7; ++j)
-            if (v[i].at && v[j].at && (intptr_t)v[i].at < (intptr_t)v[j].at + v[j].bytes && (intptr_t)v[j].at < (intptr_t)v[i].at + v[i].bytes)
+        const intptr_t a = (intptr_t)v[i].at, b = a + v[i].unit * r.n;
+        if (!a) continue;
+        for (int k = 0; k < (i < 2 ? 3 : 1); ++k) {
+            if (a >= end[k] || b <= m[k].at) continue;
+            const intptr_t off = (((a - m[k].at) % m[k].step) + m[k].step) % m[k].step;      // it may lie between two rows
+            if (off < m[k].row || off + (b - a) > m[k].step) return set_error(OB200_ERR_INVALID, "%s: %s overlaps %s", who, v[i].what, k ? "a matrix" : "grad");
+        }
+        for (int j = i + 1; i < 2 && j < 7; ++j)
+            if (v[j].at && a < (intptr_t)v[j].at + v[j].unit * r.n && (intptr_t)v[j].at < b)
                 return set_error(OB200_ERR_INVALID, "%s: %s overlaps %s", who, v[i].what, v[j].what);
     }
     return OB200_OK;
