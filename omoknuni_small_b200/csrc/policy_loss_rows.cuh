@@ -13,9 +13,11 @@
 // Rows are worked on in shared memory, where bulk copies bring them while an SM's other teams work on theirs: once for
 // the maximum (where actions that do not count are replaced by a lowest value, so that the other passes ask no mask), once
 // for the sums, once for the gradient, which leaves in 16-byte stores.  Every matrix is read from memory once and the
-// gradient written once.  Next to memory, instructions are what bounds it: at 6.5 TB/s an SM has 33 thread instructions
-// for an action of 16-bit logits with a reference row (6 bytes), 66 in fp32.  Hence the packed arithmetic (two fp32 an
-// instruction), the packed 16-bit maximum, and few threads a row, each with many actions:
+// gradient written once.  Instructions matter next to memory: at 6.5 TB/s an SM has 33 thread instructions for an action of
+// 16-bit logits with a reference row (6 bytes), 66 in fp32.  Hence the packed arithmetic (two fp32 an instruction), the
+// packed 16-bit maximum, and few threads a row, each with many actions.  No unit is full, though (1,024 x 32,768 bf16 with a
+// reference: memory 34 %, issue slots 50 %, powers of two 46 %): a row's copy, maximum, sums and gradient come one after the
+// other, and shared memory holds the rows of 20 to 24 warps an SM.
 //   policy_warp_rows_kernel   short rows: 8, 16 or 32 lanes a row, so that what a row costs besides its actions is paid
 //                             once for up to four of them
 //   policy_cta_rows_kernel    the others: a CTA or the CTAs of a cluster a row
