@@ -542,6 +542,8 @@ int32_t ob200_net_input_tensor_channels(ob200_net* net);
  * runs out: 0 = none.  Synchronises the device.  The host-buffer calls above
  * check it themselves and return OB200_ERR_TIMEOUT. */
 int ob200_device_error_code(int32_t* code_out);
+/* The same without clearing it, for a caller that is not the only one to be told. */
+int ob200_device_error_peek(int32_t* code_out);
 /* Test hook for that path: one thread waits on a barrier nobody arrives at,
  * gives up after spin_limit polls (microseconds) and raises the error word with
  * code 9.  Nothing faults or hangs; the context stays usable. */

@@ -163,6 +163,7 @@ SIGNATURES = {
     "ob200_net_value_head_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
     "ob200_value_head_noalloc_capacity": (C.c_int64, []),
     "ob200_device_error_code": (C.c_int, [C.POINTER(C.c_int32)]),
+    "ob200_device_error_peek": (C.c_int, [C.POINTER(C.c_int32)]),
     "ob200_search_create": (C.c_int, [C.c_void_p, C.POINTER(SearchConfig), C.POINTER(C.c_void_p)]),
     "ob200_search_destroy": (None, [C.c_void_p]),
     "ob200_search_run": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p,
@@ -212,9 +213,9 @@ def counters():
     return {k: getattr(c, k) for k, _ in Counters._fields_}
 
 
-def device_error_code():
+def device_error_code(clear=True):
     v = C.c_int32(0)
-    check(lib().ob200_device_error_code(C.byref(v)))
+    check((lib().ob200_device_error_code if clear else lib().ob200_device_error_peek)(C.byref(v)))
     return v.value
 
 

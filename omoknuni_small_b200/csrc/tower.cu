@@ -520,16 +520,18 @@ int ob200_debug_bounded_wait(int32_t spin_limit, ob200_stream stream) {
     return OB200_OK;
 }
 
-int ob200_device_error_code(int32_t* code_out) {
-    if (!code_out) return set_error(OB200_ERR_INVALID, "ob200_device_error_code: null output");
+static int read_error_word(const char* who, int32_t* code_out, bool clear) {
+    if (!code_out) return set_error(OB200_ERR_INVALID, "%s: null output", who);
     if (int rc = require_device()) return rc;
     int* w = device_error_word();
     if (!w) return set_error(OB200_ERR_CUDA, "cannot resolve the device error word");
     int v = 0;
     OB200_CUDA_OK(cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost));
-    if (v) { int z = 0; OB200_CUDA_OK(cudaMemcpy(w, &z, sizeof(int), cudaMemcpyHostToDevice)); }
+    if (v && clear) { int z = 0; OB200_CUDA_OK(cudaMemcpy(w, &z, sizeof(int), cudaMemcpyHostToDevice)); }
     *code_out = v;
     return OB200_OK;
 }
+int ob200_device_error_code(int32_t* code_out) { return read_error_word("ob200_device_error_code", code_out, true); }
+int ob200_device_error_peek(int32_t* code_out) { return read_error_word("ob200_device_error_peek", code_out, false); }
 
 }  // extern "C"

@@ -57,8 +57,9 @@ def check_positions(device, history, n_hist, to_move, outcome=None):
 
 class HeadLearner:
     """One optimiser over the heads of `net` (a finalised capi.Net for Gomoku) whose tensors are `weights`.  Steps run on
-    PyTorch's current stream and return without waiting; the handle may answer and search between them.  A kernel that gave
-    up on a wait makes its step's losses NaN and the step is left out; fit() and weights() report it.
+    PyTorch's current stream and return without waiting; the handle may answer and search between them.  A loss
+    kernel that gave up on a wait makes its step's losses NaN and the step is left out; fit() and weights() report that, and a
+    tower's, until capi.device_error_code() or a call of the handle has cleared the code.
 
     state_bits: AdamW states in 32 or 8 bits.  max_norm: the gradients' norm is clipped to it.  value_coef: factor of the
     squared error of the value.  The heads as they are at the start are the reference of the KL term of step_clipped."""
@@ -196,8 +197,9 @@ class HeadLearner:
         return out
 
     def _reported(self):
-        """Raises what a kernel that gave up on a wait has left on the device; steps it had a part in were left out."""
+        """Raises what a kernel that gave up on a wait has left on the device; steps it had a part in were left out.  A search
+        or an answer under way may have to read it too, so it stays."""
         with self.torch.cuda.device(self.device):
-            code = capi.device_error_code()
+            code = capi.device_error_code(clear=False)
         if code:
             raise capi.Error(capi.ERR_TIMEOUT, f"HeadLearner: a kernel gave up on a bounded wait (code {code})")

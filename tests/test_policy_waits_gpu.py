@@ -71,6 +71,9 @@ def test_learner_reports_and_leaves_the_step_out(api, no_waits):
         with pytest.raises(api.Error) as e:
             ask()
         assert e.value.code == api.ERR_TIMEOUT
+        with pytest.raises(api.Error):           # it is there for the others on the device too
+            learner.weights()
+        assert api.device_error_code(clear=False) == 4 == api.device_error_code() and api.device_error_code() == 0
         assert torch.isnan(loss).all() and torch.isnan(norm[1])
         assert all(torch.equal(p, before[k]) for k, p in learner.params.items())
     api.lib().ob200_debug_policy_waits(0)
