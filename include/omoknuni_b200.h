@@ -709,7 +709,9 @@ int ob200_copy_to_host(void* dst_host, const void* src_device, int64_t bytes);
 typedef struct ob200_policy_rows {
     const void* logits;         /* [n][logits_pitch] of dtype                     */
     const uint32_t* legal_bits; /* [n][mask_words] as ob200_tree_view, or NULL    */
-    const float* row_weight;    /* [n] factor of each row's loss; NULL = all 1    */
+    const float* row_weight;    /* [n] factor of each row's loss; NULL = all 1.  Times
+                                   (entropy_coef + kl_coef) at most 2e8: beyond it a
+                                   probability of 0 gives a gradient of NaN        */
     void* grad;                 /* [n][grad_pitch] of dtype: d loss / d logits, 0 at
                                    actions that are not legal.  May be `logits`
                                    itself (same pitch)                            */

@@ -265,3 +265,24 @@ def test_plus_infinity_makes_its_row_nan(api, dt, A, where):
     if where == "logits":
         loss, grad, stats = api.policy_loss_search(z, torch.rand((n, A), generator=g, device="cuda"), pack(legal))
         assert torch.isnan(loss[bad]).all() and torch.isnan(grad[bad]).all() and torch.isfinite(grad[~bad]).all() and torch.isfinite(loss[~bad]).all()
+
+
+@pytest.mark.parametrize("A", LENGTHS)
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_largest_weights(api, dt, A):
+    """Row weights up to the documented bound: actions that are not legal, or of logit -inf, still get a gradient of 0."""
+    import torch
+    n, T = 8, dtype_of(dt)
+    rng = np.random.default_rng(A + 5)
+    z, zr = [torch.from_numpy(rng.normal(0, 2, (n, A)).astype(np.float32)).to(T) for _ in range(2)]
+    legal = rng.random((n, A)) < 0.6
+    legal[:, 0] = True
+    z[:, A // 2] = -INF
+    w = np.full(n, 1e9, np.float32)
+    act, one = np.zeros(n, np.int32), np.ones(n, np.float32)
+    off = ~legal
+    off[:, A // 2] = True
+    for grad in (api.policy_loss_search(z.cuda(), cuda(rng.random((n, A)).astype(np.float32) * ~off), pack(legal), cuda(w), entropy_coef=0.2)[1],
+                 api.policy_loss_clipped(z.cuda(), cuda(act), cuda(-one), cuda(one), pack(legal), zr.cuda(), cuda(w), kl_coef=0.1,
+                                         entropy_coef=0.1)[1]):
+        assert torch.isfinite(grad).all() and not grad.cpu()[torch.from_numpy(off)].any() and grad[:, 0].all()
